@@ -300,7 +300,7 @@ def work(case):
     if op.startswith("norm"):
         n = case["rows"] * case["features"]
         if op == "norm_int8":
-            per = (2 * e + e if case["residual"] else e + e) + 1     # x (+ residual) -> stream, int8
+            per = (3 * e if case["residual"] else e) + 1     # x, residual -> stream, int8; without a residual x is the stream
             return {"bytes": n * per + 4 * (case["rows"] + case["features"]), "flops": 8 * n}
         # forward x, residual -> stream, y; backward stream, dy, dstream -> dx, dresidual
         return {"bytes": n * ((e + 4 + 4 + e) + (4 + e + 4 + e + 4)) + 8 * case["features"], "flops": 20 * n}
