@@ -476,6 +476,62 @@ int ssm_gated_rmsnorm_sizes(const ssm_gated_rmsnorm_params* p, size_t* workspace
 int ssm_gated_rmsnorm_fwd(const ssm_gated_rmsnorm_params* p, void* stream);
 int ssm_gated_rmsnorm_bwd(const ssm_gated_rmsnorm_params* p, void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * Residual RMSNorm, its int8 output, and the row quantiser.  No counterpart in
+ * the reference (its norm family stops at the gated RMSNorm).
+ *
+ *     s     = x + residual, rounded to stream_dtype (s = x without a residual)
+ *     y     = weight s / sqrt(mean(s^2) + eps)               (y given), or
+ *     scale = max|y| / 127,  q = rint(y / scale)             (q and scale given)
+ *
+ *   x, y, dy, dx                             : (rows, features), dtype
+ *   residual, stream, dstream, dresidual     : (rows, features), stream_dtype,
+ *                                              which is dtype or SSM_F32
+ *   weight (features): weight_dtype;  dweight (features): fp32
+ *   q (rows, features): int8;  scale, rstd (rows): fp32
+ * residual may be NULL; stream is then not written.  rstd may be NULL in the
+ * forward.  A row that holds a NaN or an infinity gets scale = NaN and q = 0; a
+ * row whose largest |weight s| is below 2^-100 gets scale = 0 and q = 0.
+ * The backward reads `stream` (x itself without a residual, with stream_dtype =
+ * dtype and x_row_stride its row stride) and rstd; dstream and dresidual may be
+ * NULL, dweight too (not written).  It takes a workspace of
+ * ssm_add_rmsnorm_sizes bytes.  dx and dresidual are the same values in the two
+ * types.  ssm_quantize_int8 uses rows, features, dtype, x_row_stride, x, q and
+ * scale: scale = max|x| / 127, q = rint(x / scale), row by row.
+ * ------------------------------------------------------------------------- */
+typedef struct ssm_add_rmsnorm_params {
+    int64_t rows, features;
+    /* elements between rows (0: features); features are contiguous in a row.
+     * stream, y, q, dx and dresidual are contiguous. */
+    int64_t x_row_stride, residual_row_stride, dy_row_stride, dstream_row_stride;
+    int32_t dtype, stream_dtype, weight_dtype;
+    float eps;
+    const void* x;
+    const void* residual;
+    const void* weight;
+    void* stream;
+    void* y;
+    int8_t* q;
+    float* scale;
+    float* rstd;
+    const void* dy;
+    const void* dstream;
+    void* dx;
+    void* dresidual;
+    float* dweight;
+    void* workspace;
+    size_t workspace_bytes;
+    /* optional device word (NULL: none), the same slot every op's params
+     * carry; this op's kernels have no waits that can give up and never
+     * write it. */
+    int32_t* status;
+} ssm_add_rmsnorm_params;
+
+int ssm_add_rmsnorm_sizes(const ssm_add_rmsnorm_params* p, size_t* workspace_bytes);
+int ssm_add_rmsnorm_fwd(const ssm_add_rmsnorm_params* p, void* stream);
+int ssm_add_rmsnorm_bwd(const ssm_add_rmsnorm_params* p, void* stream);
+int ssm_quantize_int8(const ssm_add_rmsnorm_params* p, void* stream);
+
 /* Kernels that wait on an mbarrier give up after a bounded number of polls,
  * record a non-zero code in a per-device flag (and in the call's `status`
  * word, when given) and return.  This reads the flag of the current device

@@ -47,6 +47,7 @@ EXPORTS = (
     "ssm_causal_conv1d_sizes", "ssm_causal_conv1d_fwd", "ssm_causal_conv1d_bwd",
     "ssm_causal_conv1d_update",
     "ssm_gated_rmsnorm_sizes", "ssm_gated_rmsnorm_fwd", "ssm_gated_rmsnorm_bwd",
+    "ssm_add_rmsnorm_sizes", "ssm_add_rmsnorm_fwd", "ssm_add_rmsnorm_bwd", "ssm_quantize_int8",
 )
 
 _I64, _I32, _U32, _P, _SZ = ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t
@@ -147,6 +148,19 @@ class GatedRmsNormParams(ctypes.Structure):
     ]
 
 
+class AddRmsNormParams(ctypes.Structure):
+    _fields_ = [
+        ("rows", _I64), ("features", _I64),
+        ("x_row_stride", _I64), ("residual_row_stride", _I64), ("dy_row_stride", _I64), ("dstream_row_stride", _I64),
+        ("dtype", _I32), ("stream_dtype", _I32), ("weight_dtype", _I32), ("eps", ctypes.c_float),
+        ("x", _P), ("residual", _P), ("weight", _P), ("stream", _P), ("y", _P), ("q", _P), ("scale", _P),
+        ("rstd", _P),
+        ("dy", _P), ("dstream", _P), ("dx", _P), ("dresidual", _P), ("dweight", _P),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+        ("status", _P),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -172,7 +186,8 @@ def lib():
                                  ("chunk_scan", ChunkScanParams),
                                  ("ss2d_scan", Ss2dScanParams),
                                  ("causal_conv1d", CausalConv1dParams),
-                                 ("gated_rmsnorm", GatedRmsNormParams)):
+                                 ("gated_rmsnorm", GatedRmsNormParams),
+                                 ("add_rmsnorm", AddRmsNormParams)):
                 for suffix in ("fwd", "bwd"):
                     fn = getattr(handle, f"ssm_{name}_{suffix}")
                     fn.restype = ctypes.c_int
@@ -185,6 +200,9 @@ def lib():
                 ctypes.POINTER(ChunkScanParams), ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]
             handle.ssm_causal_conv1d_sizes.argtypes = [ctypes.POINTER(CausalConv1dParams), ctypes.POINTER(_SZ)]
             handle.ssm_gated_rmsnorm_sizes.argtypes = [ctypes.POINTER(GatedRmsNormParams), ctypes.POINTER(_SZ)]
+            handle.ssm_add_rmsnorm_sizes.argtypes = [ctypes.POINTER(AddRmsNormParams), ctypes.POINTER(_SZ)]
+            handle.ssm_quantize_int8.restype = ctypes.c_int
+            handle.ssm_quantize_int8.argtypes = [ctypes.POINTER(AddRmsNormParams), ctypes.c_void_p]
             handle.ssm_causal_conv1d_update.restype = ctypes.c_int
             handle.ssm_causal_conv1d_update.argtypes = [ctypes.POINTER(CausalConv1dUpdateParams), ctypes.c_void_p]
             handle.ssm_selective_scan_fwd_workspace.argtypes = [
@@ -197,7 +215,7 @@ def lib():
                                                             ctypes.c_void_p]
             for name in ("ssm_selective_scan_sizes", "ssm_state_update_sizes", "ssm_chunk_scan_sizes",
                          "ssm_ss2d_scan_sizes", "ssm_selective_scan_fwd_workspace",
-                         "ssm_causal_conv1d_sizes", "ssm_gated_rmsnorm_sizes"):
+                         "ssm_causal_conv1d_sizes", "ssm_gated_rmsnorm_sizes", "ssm_add_rmsnorm_sizes"):
                 getattr(handle, name).restype = ctypes.c_int
             handle.ssm_take_kernel_error.restype = ctypes.c_int
             handle.ssm_take_kernel_error.argtypes = []
@@ -238,6 +256,23 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def direct(*tensors) -> bool:
+    """Whether a call without gradients may go to the library itself instead of
+    through torch's dispatcher: the tensors are plain ones (no fake or other
+    subclass) on the current device, and nothing is being traced.  The
+    dispatcher's Python path costs about 15 us a call, more than the kernels
+    of a decode step run for."""
+    if torch.compiler.is_compiling():
+        return False
+    plain = (torch.Tensor, torch.nn.Parameter)
+    return (all(t is None or type(t) in plain for t in tensors)
+            and tensors[0].get_device() == torch.cuda.current_device())
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 # --------------------------------------------------------------- status words --
 # One int32 device word per op family and device, zero-initialised once from
 # the caching allocator and handed to every call of that op (params.status).
@@ -245,7 +280,7 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
 # cleared until ``check_errors`` reads the words.  Reading is lazy -- one small
 # device-to-host copy when the caller asks -- so the ops never synchronise.
 STATUS_SLOTS = ("selective_scan", "state_update", "chunk_scan", "ss2d_scan", "causal_conv1d",
-                "causal_conv1d_update", "gated_rmsnorm", "selftest")
+                "causal_conv1d_update", "gated_rmsnorm", "selftest", "add_rmsnorm", "int8_linear", "gated_recurrence")
 _status = {}
 
 

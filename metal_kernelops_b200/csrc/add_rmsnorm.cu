@@ -1,0 +1,585 @@
+// Residual RMSNorm with an optional int8 output, its backward pass, and the
+// row quantiser that shares its last step.
+//
+// Per row of F features, in fp32:
+//     s     = x + residual, rounded to the residual stream's type (s = x without one)
+//     rstd  = 1 / sqrt(mean(s^2) + eps),   y = w s rstd
+//     int8: scale = max|y| / 127,  q = rint(y / scale)
+// The norm reads s as it is stored, so that the backward pass, and a layer run
+// again from the stored stream, see the very values the forward saw.
+// max|y| = rstd max|w s| and y / scale = 127 w s / max|w s|, so the sum of
+// squares and the maximum come from one pass over the row and one reduction.
+// The maximum is taken over the bit patterns of |w s| as unsigned integers: for
+// non-negative floats their order is the values' order, with infinities and then
+// NaN above every finite value, so a row that holds one is recognised; its scale
+// is NaN and its q zero, and what reads it is NaN rather than silently finite.
+// Rows whose largest |y| (before the factor rstd) is below 2^-100 count as zero.
+// Backward, with xh = s rstd and c = mean(w dy xh):
+//     d  = rstd (w dy - xh c) + dstream,   dx = dresidual = d,   dw = sum_rows dy xh
+//
+// Bytes bound these kernels: each row is read once and kept in registers.  A row
+// belongs to a group of `tx` threads (whole warps; tx NV vectors of 8 elements
+// cover the row), a CTA holds several rows when they are narrow.  The backward
+// CTAs walk rows blockIdx, blockIdx + grid, ..., keep their columns' dw sums in
+// registers and leave one partial row each; the fold adds the partials in a
+// fixed order, so results are reproducible.  Rows whose width or alignment does
+// not allow 8-element vectors, and rows above 16384 features (8192 in the
+// backward), stream: a CTA reads such a row twice, the second time from L1 / L2.
+#include <climits>
+
+#include "common.cuh"
+
+namespace ssm {
+namespace anorm {
+
+constexpr int kMaxThreads = 512;
+constexpr int kMaxWarps = kMaxThreads / 32;
+constexpr float kTiny = 7.888609052210118e-31f;     // 2^-100
+
+struct Args {
+    int64_t rows, features, xs, rs;          // rs: residual row stride
+    float eps, inv_f;
+    int weight_dtype;
+    const void* x; const void* res; const void* w;
+    void* stream; void* y; int8_t* q; float* scale; float* rstd;
+    const void* dy; const void* ds; void* dx; void* dres; float* part;
+    int64_t dys, dss;
+};
+
+// Eight consecutive elements.
+template <typename T> struct V8;
+template <> struct V8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void ld(const float* p) {
+        a = reinterpret_cast<const float4*>(p)[0];
+        b = reinterpret_cast<const float4*>(p)[1];
+    }
+    __device__ __forceinline__ void get(float* v) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    __device__ __forceinline__ void set(const float* v) {
+        a = make_float4(v[0], v[1], v[2], v[3]);
+        b = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    __device__ __forceinline__ void st(float* p) const {
+        reinterpret_cast<float4*>(p)[0] = a;
+        reinterpret_cast<float4*>(p)[1] = b;
+    }
+};
+template <typename T, typename H2> struct V8h {
+    uint4 r;
+    __device__ __forceinline__ void ld(const T* p) { r = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void get(float* v) const {
+        const T* h = reinterpret_cast<const T*>(&r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = Io2<T>::ld(h + 2 * i);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+    __device__ __forceinline__ void set(const float* v) {
+        T* h = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Io2<T>::st(h + 2 * i, make_float2(v[2 * i], v[2 * i + 1]));
+    }
+    __device__ __forceinline__ void st(T* p) const { *reinterpret_cast<uint4*>(p) = r; }
+};
+template <> struct V8<__nv_bfloat16> : V8h<__nv_bfloat16, __nv_bfloat162> {};
+template <> struct V8<__half> : V8h<__half, __half2> {};
+
+template <typename TS> __device__ __forceinline__ float as_stored(float v);
+template <> __device__ __forceinline__ float as_stored<float>(float v) { return v; }
+template <> __device__ __forceinline__ float as_stored<__nv_bfloat16>(float v) {
+    return __bfloat162float(__float2bfloat16_rn(v));
+}
+template <> __device__ __forceinline__ float as_stored<__half>(float v) { return __half2float(__float2half_rn(v)); }
+
+__device__ __forceinline__ void ld_weight8(const Args& a, int64_t e, float* w) {
+    if (a.weight_dtype == SSM_F32) {
+        V8<float> v; v.ld(static_cast<const float*>(a.w) + e); v.get(w);
+    } else if (a.weight_dtype == SSM_BF16) {
+        V8<__nv_bfloat16> v; v.ld(static_cast<const __nv_bfloat16*>(a.w) + e); v.get(w);
+    } else {
+        V8<__half> v; v.ld(static_cast<const __half*>(a.w) + e); v.get(w);
+    }
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Sum and maximum over the `warps` warps that share a row; `red` holds them.
+// Every thread of the CTA calls it the same number of times.
+struct SumMax { float sum; uint32_t mx; };
+__device__ __forceinline__ SumMax row_reduce(SumMax v, int warps, SumMax* red) {
+    v.sum = sum_low_lanes<32>(v.sum);
+    v.mx = __reduce_max_sync(0xffffffffu, v.mx);
+    if (warps == 1) return v;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    SumMax* mine = red + threadIdx.y * warps;
+    if (lane == 0) mine[warp] = v;
+    __syncthreads();
+    v = mine[0];
+    for (int i = 1; i < warps; ++i) {
+        v.sum += mine[i].sum;
+        v.mx = v.mx > mine[i].mx ? v.mx : mine[i].mx;
+    }
+    return v;
+}
+
+// The int8 step's factors from max|v| of a row (as bits): v * inv rounds to q,
+// and q * scale1 stands for v.
+struct Quant { float inv, scale1; };
+__device__ __forceinline__ Quant quant_of(uint32_t mx) {
+    const float m = __uint_as_float(mx);
+    if (mx >= 0x7f800000u) return {0.0f, __uint_as_float(0x7fc00000u)};
+    if (m < kTiny) return {0.0f, 0.0f};
+    return {127.0f / m, m / 127.0f};
+}
+// rint(v * inv) in the low byte: adding 1.5 * 2^23 leaves the rounded integer
+// (to nearest, ties to even) in the low bits of the sum.
+__device__ __forceinline__ uint32_t q_bits(float v, float inv) {
+    return __float_as_uint(fmaf(v, inv, 12582912.0f));
+}
+// A row that is not finite has inv = 0 and must store zeros, also where v is
+// infinite or NaN.
+__device__ __forceinline__ uint32_t pack4(const float* v, float inv) {
+    const uint32_t lo = __byte_perm(q_bits(v[0], inv), q_bits(v[1], inv), 0x0040);
+    const uint32_t hi = __byte_perm(q_bits(v[2], inv), q_bits(v[3], inv), 0x0040);
+    return inv != 0.0f ? __byte_perm(lo, hi, 0x5410) : 0u;
+}
+
+// x (+ residual) -> s, and s stored; the eight s values.
+template <typename T, typename TS>
+__device__ __forceinline__ void sum8(const Args& a, int64_t row, int64_t e, const V8<T>& xr, const V8<TS>& rr,
+                                     float* v) {
+    xr.get(v);
+    if (a.res != nullptr) {
+        float r[8];
+        rr.get(r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] + r[i];
+        V8<TS> s;
+        s.set(v);
+        s.get(v);
+        s.st(static_cast<TS*>(a.stream) + row * a.features + e);
+    }
+}
+
+enum Mode { kNorm, kNormInt8, kInt8 };    // y, q and scale, q and scale of x itself
+
+template <typename T, typename TS, int NV, int MODE>
+__global__ void __launch_bounds__(kMaxThreads)
+fwd_kernel(const Args a) {
+    __shared__ SumMax red[kMaxWarps];
+    const int64_t F = a.features;
+    const int tx = blockDim.x, warps = tx >> 5;
+    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const bool live = row < a.rows;
+    float v[NV][8];
+    V8<T> xr[NV];
+    V8<TS> rr[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+        if (live && e < F) {
+            xr[k].ld(static_cast<const T*>(a.x) + row * a.xs + e);
+            if (MODE != kInt8 && a.res != nullptr) rr[k].ld(static_cast<const TS*>(a.res) + row * a.rs + e);
+        }
+    }
+    SumMax sm{0.0f, 0u};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+        if (live && e < F) {
+            if (MODE == kInt8) {
+                xr[k].get(v[k]);
+            } else {
+                float w[8];
+                ld_weight8(a, e, w);
+                sum8<T, TS>(a, row, e, xr[k], rr[k], v[k]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    sm.sum = fmaf(v[k][i], v[k][i], sm.sum);
+                    v[k][i] *= w[i];
+                }
+            }
+            if (MODE != kNorm) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sm.mx = max(sm.mx, abs_bits(v[k][i]));
+            }
+        }
+    }
+    sm = row_reduce(sm, warps, red);
+    if (!live) return;
+    const float r = MODE == kInt8 ? 1.0f : 1.0f / sqrtf(fmaf(sm.sum, a.inv_f, a.eps));
+    if (MODE == kNorm) {
+        if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = r;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+            if (e < F) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[k][i] *= r;
+                V8<T> o;
+                o.set(v[k]);
+                o.st(static_cast<T*>(a.y) + row * F + e);
+            }
+        }
+    } else {
+        const Quant qt = quant_of(sm.mx);
+        if (threadIdx.x == 0) a.scale[row] = qt.scale1 * r;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+            if (e < F)
+                *reinterpret_cast<uint2*>(a.q + row * F + e) =
+                    make_uint2(pack4(v[k], qt.inv), pack4(v[k] + 4, qt.inv));
+        }
+    }
+}
+
+// One row per CTA, element by element, in two passes over the row.
+template <typename T, typename TS, int MODE>
+__global__ void __launch_bounds__(kMaxThreads)
+fwd_stream_kernel(const Args a) {
+    __shared__ SumMax red[kMaxWarps];
+    const int64_t F = a.features, row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    const TS* res = a.res != nullptr ? static_cast<const TS*>(a.res) + row * a.rs : nullptr;
+    TS* stream = static_cast<TS*>(a.stream) + (res ? row * F : 0);
+    auto value = [&](int64_t e) {
+        float v = ldf(x + e);
+        return res ? as_stored<TS>(v + ldf(res + e)) : v;
+    };
+    SumMax sm{0.0f, 0u};
+    for (int64_t e = threadIdx.x; e < F; e += blockDim.x) {
+        float v = MODE == kInt8 ? ldf(x + e) : value(e);
+        if (MODE != kInt8) {
+            if (res) stf(stream + e, v);
+            sm.sum = fmaf(v, v, sm.sum);
+            v *= ld_any(a.w, e, a.weight_dtype);
+        }
+        if (MODE != kNorm) sm.mx = max(sm.mx, abs_bits(v));
+    }
+    sm = row_reduce(sm, blockDim.x >> 5, red);
+    const float r = MODE == kInt8 ? 1.0f : 1.0f / sqrtf(fmaf(sm.sum, a.inv_f, a.eps));
+    const Quant qt = quant_of(sm.mx);
+    if (threadIdx.x == 0) {
+        if (MODE != kNorm) a.scale[row] = qt.scale1 * r;
+        else if (a.rstd != nullptr) a.rstd[row] = r;
+    }
+    for (int64_t e = threadIdx.x; e < F; e += blockDim.x) {
+        float v = MODE == kInt8 ? ldf(x + e) : value(e);
+        if (MODE != kInt8) v *= ld_any(a.w, e, a.weight_dtype);
+        if (MODE == kNorm) stf(static_cast<T*>(a.y) + row * F + e, v * r);
+        else a.q[row * F + e] = qt.inv != 0.0f ? (int8_t)(q_bits(v, qt.inv) & 0xffu) : (int8_t)0;
+    }
+}
+
+template <typename T, typename TS, int NV>
+__global__ void __launch_bounds__(kMaxThreads)
+bwd_kernel(const Args a) {
+    __shared__ SumMax red[2][kMaxWarps];
+    const int64_t F = a.features;
+    const int tx = blockDim.x, warps = tx >> 5;
+    const TS* s = static_cast<const TS*>(a.stream);
+    const T* dy = static_cast<const T*>(a.dy);
+    const TS* ds = static_cast<const TS*>(a.ds);
+    float dw[NV][8] = {};
+    float w[NV][8] = {};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+        if (e < F) ld_weight8(a, e, w[k]);
+    }
+    const int64_t step = (int64_t)gridDim.x * blockDim.y;
+    int turn = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * blockDim.y; r0 < a.rows; r0 += step, turn ^= 1) {
+        const int64_t row = r0 + threadIdx.y;
+        const bool live = row < a.rows;
+        V8<TS> sr[NV], dsr[NV];
+        V8<T> dyr[NV];
+        float rstd = 0.0f;
+        if (live) {
+            rstd = a.rstd[row];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+                if (e < F) {
+                    sr[k].ld(s + row * a.xs + e);
+                    if (dy) dyr[k].ld(dy + row * a.dys + e);
+                    if (ds) dsr[k].ld(ds + row * a.dss + e);
+                }
+            }
+        }
+        SumMax c{0.0f, 0u};
+        float xh[NV][8], g[NV][8];
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+                if (e < F) {
+                    sr[k].get(xh[k]);
+                    dyr[k].get(g[k]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        xh[k][i] *= rstd;
+                        dw[k][i] = fmaf(g[k][i], xh[k][i], dw[k][i]);
+                        g[k][i] *= w[k][i];
+                        c.sum = fmaf(g[k][i], xh[k][i], c.sum);
+                    }
+                }
+            }
+        }
+        const float c1 = row_reduce(c, warps, red[turn]).sum * a.inv_f;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+                if (e < F) {
+                    float d[8];
+                    if (ds) dsr[k].get(d);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[i] = fmaf(rstd, fmaf(-xh[k][i], c1, g[k][i]), ds ? d[i] : 0.0f);
+                    V8<T> o;
+                    o.set(d);
+                    o.st(static_cast<T*>(a.dx) + row * F + e);
+                    if (a.dres) {
+                        V8<TS> p;
+                        p.set(d);
+                        p.st(static_cast<TS*>(a.dres) + row * F + e);
+                    }
+                }
+            }
+        }
+    }
+    if (a.part == nullptr) return;
+    float* part = a.part + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * F;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+        if (e < F) {
+            V8<float> o;
+            o.set(dw[k]);
+            o.st(part + e);
+        }
+    }
+}
+
+// Element by element; the CTA's dw partial lives in its own row of `part`.
+template <typename T, typename TS>
+__global__ void __launch_bounds__(kMaxThreads)
+bwd_stream_kernel(const Args a) {
+    __shared__ SumMax red[2][kMaxWarps];
+    const int64_t F = a.features;
+    float* part = a.part + blockIdx.x * F;
+    for (int64_t e = threadIdx.x; e < F; e += blockDim.x) part[e] = 0.0f;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const TS* s = static_cast<const TS*>(a.stream) + row * a.xs;
+        const T* dy = static_cast<const T*>(a.dy) + row * a.dys;
+        const TS* ds = a.ds ? static_cast<const TS*>(a.ds) + row * a.dss : nullptr;
+        const float rstd = a.rstd[row];
+        SumMax c{0.0f, 0u};
+        for (int64_t e = threadIdx.x; e < F; e += blockDim.x) {
+            const float xh = ldf(s + e) * rstd, up = ldf(dy + e);
+            part[e] = fmaf(up, xh, part[e]);
+            c.sum = fmaf(up * ld_any(a.w, e, a.weight_dtype), xh, c.sum);
+        }
+        const float c1 = row_reduce(c, blockDim.x >> 5, red[turn]).sum * a.inv_f;
+        for (int64_t e = threadIdx.x; e < F; e += blockDim.x) {
+            const float xh = ldf(s + e) * rstd, g = ldf(dy + e) * ld_any(a.w, e, a.weight_dtype);
+            const float d = fmaf(rstd, fmaf(-xh, c1, g), ds ? ldf(ds + e) : 0.0f);
+            stf(static_cast<T*>(a.dx) + row * F + e, d);
+            if (a.dres) stf(static_cast<TS*>(a.dres) + row * F + e, d);
+        }
+    }
+}
+
+// dw[f] = the partial rows added in order: 32 columns a CTA, eight runs of
+// consecutive partial rows each summed by one warp, the runs added in order.
+__global__ void __launch_bounds__(256) fold_kernel(const float* part, int64_t parts, int64_t F, float* dw) {
+    __shared__ float run[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t f = (int64_t)blockIdx.x * 32 + lane;
+    const int64_t per = (parts + 7) / 8, k0 = warp * per, k1 = min64(k0 + per, parts);
+    float s = 0.0f;
+    if (f < F)
+        for (int64_t k = k0; k < k1; ++k) s += part[k * F + f];
+    run[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && f < F) {
+        s = run[0][lane];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += run[i][lane];
+        dw[f] = s;
+    }
+}
+
+// ------------------------------------------------------------------- host ----
+static bool al(const void* p, int64_t b) { return (reinterpret_cast<uintptr_t>(p) % b) == 0; }
+static int64_t esize(int dtype) { return dtype == SSM_F32 ? 4 : 2; }
+
+// The widest rows that a CTA's registers hold: 512 threads x 32 elements in the
+// forward; x 16 in the backward, which also keeps the weights and their sums.
+constexpr int64_t kMaxFwd = kMaxThreads * 32, kMaxBwd = kMaxThreads * 16;
+
+// nv = 0: the streaming kernels.
+struct Shape { int tx, ty, nv; };
+
+static Shape shape_of(int64_t F, bool vec, bool bwd) {
+    if (!vec || F > (bwd ? kMaxBwd : kMaxFwd)) return {(int)min64(kMaxThreads, ceil_div(F, 32) * 32), 1, 0};
+    const int64_t n = F / 8;
+    const int nv = n <= 512 ? 1 : n <= 1024 ? 2 : 4;
+    const int tx = (int)(ceil_div(ceil_div(n, nv), 32) * 32);
+    return {tx, tx >= 128 ? 1 : 128 / tx, nv};
+}
+
+static int validate(const ssm_add_rmsnorm_params* p, const char* op) {
+    if (p == nullptr) return fail(SSM_ERR_INVALID, std::string(op) + ": null params");
+    if (p->rows < 0 || p->features < 1) return fail(SSM_ERR_INVALID, std::string(op) + ": rows and features");
+    if (p->rows > INT32_MAX || p->features > INT32_MAX)
+        return fail(SSM_ERR_UNSUPPORTED, std::string(op) + ": more than 2^31 - 1 rows or features");
+    if (p->dtype < SSM_F32 || p->dtype > SSM_F16 || p->weight_dtype < SSM_F32 || p->weight_dtype > SSM_F16)
+        return fail(SSM_ERR_UNSUPPORTED, std::string(op) + ": dtype");
+    if (p->stream_dtype != p->dtype && p->stream_dtype != SSM_F32)
+        return fail(SSM_ERR_UNSUPPORTED, std::string(op) + ": the residual stream has x's dtype or float32");
+    for (int64_t st : {p->x_row_stride, p->residual_row_stride, p->dy_row_stride, p->dstream_row_stride})
+        if (st && st < p->features) return fail(SSM_ERR_INVALID, std::string(op) + ": a row stride is below features");
+    return SSM_OK;
+}
+
+static Args args_of(const ssm_add_rmsnorm_params* p) {
+    Args a{};
+    a.rows = p->rows; a.features = p->features;
+    a.xs = p->x_row_stride ? p->x_row_stride : p->features;
+    a.rs = p->residual_row_stride ? p->residual_row_stride : p->features;
+    a.dys = p->dy_row_stride ? p->dy_row_stride : p->features;
+    a.dss = p->dstream_row_stride ? p->dstream_row_stride : p->features;
+    a.eps = p->eps;
+    a.inv_f = 1.0f / (float)p->features;
+    a.weight_dtype = p->weight_dtype;
+    a.x = p->x; a.res = p->residual; a.w = p->weight;
+    a.stream = p->stream; a.y = p->y; a.q = p->q; a.scale = p->scale; a.rstd = p->rstd;
+    a.dy = p->dy; a.ds = p->dstream; a.dx = p->dx; a.dres = p->dresidual;
+    return a;
+}
+
+template <typename T, typename TS, int MODE>
+static int launch_fwd(const Args& a, const Shape& s, cudaStream_t st) {
+    const dim3 block(s.tx, s.ty);
+    const unsigned grid = (unsigned)ceil_div(a.rows, s.ty);
+    switch (s.nv) {
+        case 0: fwd_stream_kernel<T, TS, MODE><<<grid, block, 0, st>>>(a); break;
+        case 1: fwd_kernel<T, TS, 1, MODE><<<grid, block, 0, st>>>(a); break;
+        case 2: fwd_kernel<T, TS, 2, MODE><<<grid, block, 0, st>>>(a); break;
+        default: fwd_kernel<T, TS, 4, MODE><<<grid, block, 0, st>>>(a);
+    }
+    return check_launch(MODE == kInt8 ? "quantize_int8" : "add_rmsnorm fwd");
+}
+
+template <int MODE>
+static int dispatch_fwd(const Args& a, const Shape& s, int dtype, int stream_dtype, cudaStream_t st) {
+    if (dtype == SSM_F32) return launch_fwd<float, float, MODE>(a, s, st);
+    if (dtype == SSM_BF16) {
+        if (MODE == kInt8 || stream_dtype == SSM_BF16) return launch_fwd<__nv_bfloat16, __nv_bfloat16, MODE>(a, s, st);
+        return launch_fwd<__nv_bfloat16, float, MODE>(a, s, st);
+    }
+    if (MODE == kInt8 || stream_dtype == SSM_F16) return launch_fwd<__half, __half, MODE>(a, s, st);
+    return launch_fwd<__half, float, MODE>(a, s, st);
+}
+
+// Whether every tensor the forward touches allows 8-element vectors.
+static bool vec_fwd(const ssm_add_rmsnorm_params* p, const Args& a, bool quant_only) {
+    const int64_t e = esize(p->dtype), es = esize(p->stream_dtype);
+    if (a.features % 8 || !al(a.x, 16) || (a.xs * e) % 16 || !al(a.q, 8) || !al(a.y, 16)) return false;
+    if (quant_only) return true;
+    if (!al(a.w, 16)) return false;
+    return !a.res || (al(a.res, 16) && (a.rs * es) % 16 == 0 && al(a.stream, 16));
+}
+
+// Backward CTAs: rows in turn over up to two CTAs per SM.
+static int64_t bwd_ctas(int64_t rows, int ty) { return min64(ceil_div(max64(rows, 1), ty), 148 * 2); }
+
+template <typename T, typename TS>
+static void launch_bwd(const Args& a, const Shape& s, int64_t ctas, cudaStream_t st) {
+    const dim3 block(s.tx, s.ty);
+    switch (s.nv) {
+        case 0: bwd_stream_kernel<T, TS><<<(unsigned)ctas, block, 0, st>>>(a); break;
+        case 1: bwd_kernel<T, TS, 1><<<(unsigned)ctas, block, 0, st>>>(a); break;
+        default: bwd_kernel<T, TS, 2><<<(unsigned)ctas, block, 0, st>>>(a);
+    }
+}
+
+}  // namespace anorm
+}  // namespace ssm
+
+using namespace ssm;
+using namespace ssm::anorm;
+
+extern "C" int ssm_add_rmsnorm_sizes(const ssm_add_rmsnorm_params* p, size_t* workspace_bytes) {
+    if (int s = validate(p, "add_rmsnorm")) return s;
+    // either kernel's partial rows (the vector kernels leave one per row group)
+    const Shape sh = shape_of(p->features, p->features % 8 == 0, true);
+    const int64_t parts = max64(bwd_ctas(p->rows, sh.ty) * sh.ty, bwd_ctas(p->rows, 1));
+    if (workspace_bytes) *workspace_bytes = (size_t)(parts * p->features) * 4;
+    return SSM_OK;
+}
+
+extern "C" int ssm_add_rmsnorm_fwd(const ssm_add_rmsnorm_params* p, void* stream) {
+    if (int s = validate(p, "add_rmsnorm")) return s;
+    if (p->rows == 0) return SSM_OK;
+    if (!p->x || !p->weight || (p->residual && !p->stream) || !(p->y || (p->q && p->scale)))
+        return fail(SSM_ERR_INVALID, "add_rmsnorm fwd: null pointer");
+    if (p->y && p->q) return fail(SSM_ERR_INVALID, "add_rmsnorm fwd: y and q are alternatives");
+    const Args a = args_of(p);
+    const Shape sh = shape_of(a.features, vec_fwd(p, a, false), false);
+    const int sd = p->residual ? p->stream_dtype : p->dtype;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return p->q ? dispatch_fwd<kNormInt8>(a, sh, p->dtype, sd, st) : dispatch_fwd<kNorm>(a, sh, p->dtype, sd, st);
+}
+
+extern "C" int ssm_quantize_int8(const ssm_add_rmsnorm_params* p, void* stream) {
+    if (int s = validate(p, "quantize_int8")) return s;
+    if (p->rows == 0) return SSM_OK;
+    if (!p->x || !p->q || !p->scale) return fail(SSM_ERR_INVALID, "quantize_int8: null pointer");
+    const Args a = args_of(p);
+    return dispatch_fwd<kInt8>(a, shape_of(a.features, vec_fwd(p, a, true), false), p->dtype, p->dtype,
+                               static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ssm_add_rmsnorm_bwd(const ssm_add_rmsnorm_params* p, void* stream) {
+    if (int s = validate(p, "add_rmsnorm")) return s;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p->rows == 0) {
+        if (p->dweight && cudaMemsetAsync(p->dweight, 0, (size_t)p->features * 4, st))
+            return check_launch("add_rmsnorm bwd: zero dweight");
+        return SSM_OK;
+    }
+    if (!p->stream || !p->weight || !p->dy || !p->rstd || !p->dx)
+        return fail(SSM_ERR_INVALID, "add_rmsnorm bwd: null pointer");
+    size_t need = 0;
+    ssm_add_rmsnorm_sizes(p, &need);
+    if (!p->workspace || p->workspace_bytes < need)
+        return fail(SSM_ERR_WORKSPACE, "add_rmsnorm bwd: workspace smaller than ssm_add_rmsnorm_sizes");
+    Args a = args_of(p);
+    a.part = static_cast<float*>(p->workspace);
+    const int64_t e = esize(p->dtype), es = esize(p->stream_dtype);
+    // x_row_stride is the saved stream's here
+    const bool vec = a.features % 8 == 0 && al(a.stream, 16) && (a.xs * es) % 16 == 0 && al(a.w, 16) &&
+                     al(a.dy, 16) && (a.dys * e) % 16 == 0 && al(a.dx, 16) && al(a.part, 16) &&
+                     (!a.ds || (al(a.ds, 16) && (a.dss * es) % 16 == 0)) && (!a.dres || al(a.dres, 16));
+    const Shape sh = shape_of(a.features, vec, true);
+    const int64_t ctas = bwd_ctas(a.rows, sh.ty);
+    if (p->dtype == SSM_F32) launch_bwd<float, float>(a, sh, ctas, st);
+    else if (p->dtype == SSM_BF16 && p->stream_dtype == SSM_BF16) launch_bwd<__nv_bfloat16, __nv_bfloat16>(a, sh, ctas, st);
+    else if (p->dtype == SSM_BF16) launch_bwd<__nv_bfloat16, float>(a, sh, ctas, st);
+    else if (p->stream_dtype == SSM_F16) launch_bwd<__half, __half>(a, sh, ctas, st);
+    else launch_bwd<__half, float>(a, sh, ctas, st);
+    if (int s = check_launch("add_rmsnorm bwd")) return s;
+    if (p->dweight) {
+        fold_kernel<<<(unsigned)ceil_div(a.features, 32), 256, 0, st>>>(a.part, ctas * sh.ty, a.features, p->dweight);
+        return check_launch("add_rmsnorm bwd: fold");
+    }
+    return SSM_OK;
+}

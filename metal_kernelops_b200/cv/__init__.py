@@ -9,15 +9,21 @@
 * ``rmsnorm_gated`` -- gated RMSNorm, mamba's ``rms_norm_ref``
   (cv/gated_norm.py:647-686)
 
+Language-model operators around the scans (no counterpart in the reference):
+
+* ``add_rmsnorm``, ``add_rmsnorm_int8``, ``quantize_int8`` -- residual RMSNorm,
+  its int8 output, and the row quantiser
+
 The reference's other ``cv`` families (NSA selection, RoIAlign) are outside
 this package's scope.
 """
 
+from .add_rmsnorm import add_rmsnorm, add_rmsnorm_int8, quantize_int8
 from .causal_conv1d import causal_conv1d_fn, causal_conv1d_update
 from .gated_norm import rmsnorm_gated
 from .mamba2_chunk import last_path, mamba2_chunk_scan, tc_shape
 from .mamba2_state import mamba2_state_update
 from .path_scan import path_orders, ss2d_scan
 
-__all__ = ["causal_conv1d_fn", "causal_conv1d_update", "last_path", "mamba2_chunk_scan",
+__all__ = ["add_rmsnorm", "add_rmsnorm_int8", "quantize_int8", "causal_conv1d_fn", "causal_conv1d_update", "last_path", "mamba2_chunk_scan",
            "mamba2_state_update", "path_orders", "rmsnorm_gated", "ss2d_scan", "tc_shape"]

@@ -1,0 +1,248 @@
+"""Residual RMSNorm on the B200, with an int8 output for the int8 projections.
+
+The pre-norm of a residual layer: the mixer's output joins the residual stream
+and the next layer reads the normalised stream,
+
+    stream = x + residual                      (x itself without a residual)
+    y      = weight * stream / sqrt(mean(stream^2) + eps)
+
+over the last axis, all arithmetic in float32.  ``stream`` is in the residual's
+dtype (float32, or x's), and the norm reads it as stored.  x may be float32,
+bfloat16 or float16 with any leading shape, weight any of the three.
+
+* :func:`add_rmsnorm` returns ``(y, stream)`` with y in x's dtype, and has a
+  backward pass (x, residual and weight).
+* :func:`add_rmsnorm_int8` returns ``(q, scale, stream)``: y as int8 rows with
+  one float32 scale a row, ``scale = max|y| / 127``, ``q = rint(y / scale)``.
+* :func:`quantize_int8` does the same to the rows of a tensor as it is: the
+  activations of a projection that follows no norm, or a weight matrix (one
+  scale per output channel).
+
+A row that holds a NaN or an infinity has scale NaN (what reads it is NaN, not
+silently finite); a row of zeros has scale 0.  The int8 functions have no
+gradient and say so when one is asked for.  The reference has no counterpart.
+CUDA tensors only; kernels in ``csrc/add_rmsnorm.cu``.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import _native as nat
+from .gated_norm import _rows
+
+__all__ = ["add_rmsnorm", "add_rmsnorm_int8", "quantize_int8"]
+
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _stride(t):
+    return t.stride(0) if t is not None and t.shape[0] > 1 else 0
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _params(x, residual, weight, eps, stream=None, y=None, q=None, scale=None, rstd=None):
+    stream_dtype = x.dtype if residual is None else residual.dtype
+    return nat.AddRmsNormParams(
+        x.shape[0], x.shape[1], _stride(x), _stride(residual), 0, 0, nat.dtype_code(x.dtype),
+        nat.dtype_code(stream_dtype), 0 if weight is None else nat.dtype_code(weight.dtype), eps, x.data_ptr(),
+        _ptr(residual), _ptr(weight), _ptr(stream), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
+
+
+def _forward(x, weight, residual, eps, save):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stream = torch.empty(x.shape if residual is not None else (0,),
+                         dtype=x.dtype if residual is None else residual.dtype, device=x.device)
+    rstd = torch.empty(x.shape[0] if save else 0, dtype=torch.float32, device=x.device)
+    p = _params(x, residual, weight, eps, stream if residual is not None else None, y, rstd=rstd if save else None)
+    nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_of(x)), "add_rmsnorm")
+    return y, stream, rstd
+
+
+def _forward_int8(x, weight, residual, eps):
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+    stream = torch.empty(x.shape if residual is not None else (0,),
+                         dtype=x.dtype if residual is None else residual.dtype, device=x.device)
+    p = _params(x, residual, weight, eps, stream if residual is not None else None, q=q, scale=scale)
+    nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_of(x)), "add_rmsnorm_int8")
+    return q, scale, stream
+
+
+def _quantize(x):
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+    p = _params(x, None, None, 0.0, q=q, scale=scale)
+    nat.check(nat.lib().ssm_quantize_int8(p, nat.stream_of(x)), "quantize_int8")
+    return q, scale
+
+
+@torch.library.custom_op("b200ssm::add_rmsnorm_fwd", mutates_args=(), device_types="cuda")
+def _fwd(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor], eps: float,
+         save: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _forward(x, weight, residual, eps, save)
+
+
+@_fwd.register_fake
+def _(x, weight, residual, eps, save):
+    return (x.new_empty(x.shape), x.new_empty(0) if residual is None else residual.new_empty(x.shape),
+            x.new_empty(x.shape[0] if save else 0, dtype=torch.float32))
+
+
+@torch.library.custom_op("b200ssm::add_rmsnorm_int8", mutates_args=(), device_types="cuda")
+def _int8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor],
+          eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _forward_int8(x, weight, residual, eps)
+
+
+@_int8.register_fake
+def _(x, weight, residual, eps):
+    return (x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[0], dtype=torch.float32),
+            x.new_empty(0) if residual is None else residual.new_empty(x.shape))
+
+
+@torch.library.custom_op("b200ssm::quantize_int8", mutates_args=(), device_types="cuda")
+def _quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return _quantize(x)
+
+
+@_quant.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[0], dtype=torch.float32)
+
+
+@torch.library.custom_op("b200ssm::add_rmsnorm_bwd", mutates_args=(), device_types="cuda")
+def _bwd(dy: torch.Tensor, dstream: Optional[torch.Tensor], stream: torch.Tensor, weight: torch.Tensor,
+         rstd: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    rows, features = dy.shape
+    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    both = stream.dtype != dy.dtype                 # the stream's gradient in its own type
+    dres = torch.empty(dy.shape if both else (0,), dtype=stream.dtype, device=dy.device)
+    dw = torch.empty(features, dtype=torch.float32, device=dy.device)
+    p = nat.AddRmsNormParams(
+        rows, features, _stride(stream), 0, _stride(dy), _stride(dstream), nat.dtype_code(dy.dtype),
+        nat.dtype_code(stream.dtype), nat.dtype_code(weight.dtype), eps)
+    need = nat._SZ()
+    nat.check(nat.lib().ssm_add_rmsnorm_sizes(p, need), "add_rmsnorm backward")
+    ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=dy.device)
+    p.stream, p.weight, p.rstd, p.dy, p.dx = (t.data_ptr() for t in (stream, weight, rstd, dy, dx))
+    p.dstream, p.dresidual, p.dweight = _ptr(dstream), dres.data_ptr() if both else None, dw.data_ptr()
+    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+    nat.check(nat.lib().ssm_add_rmsnorm_bwd(p, nat.stream_of(dy)), "add_rmsnorm backward")
+    return dx, dres, dw
+
+
+@_bwd.register_fake
+def _(dy, dstream, stream, weight, rstd, eps):
+    return (dy.new_empty(dy.shape), stream.new_empty(dy.shape if stream.dtype != dy.dtype else (0,)),
+            dy.new_empty(dy.shape[1], dtype=torch.float32))
+
+
+def _setup(ctx, inputs, output):
+    x, weight, residual, eps, save = inputs
+    _, stream, rstd = output
+    ctx.save_for_backward(x if residual is None else stream, weight, rstd)
+    ctx.eps, ctx.residual, ctx.xdtype = eps, residual is not None, x.dtype
+    ctx.set_materialize_grads(False)
+
+
+def _backward(ctx, dy, dstream, drstd):
+    stream, weight, rstd = ctx.saved_tensors
+    if rstd.numel() == 0 and stream.numel():
+        raise RuntimeError("add_rmsnorm: the forward did not save its statistics (save=False)")
+    if dy is None and dstream is None:
+        return (None,) * 5
+    dstream = _rows(dstream, stream.shape[1]) if ctx.residual and dstream is not None else None
+    dy = torch.zeros(stream.shape, dtype=ctx.xdtype, device=stream.device) if dy is None else _rows(dy, stream.shape[1])
+    dx, dres, dw = _bwd(dy, dstream, stream, weight, rstd, ctx.eps)
+    dres = None if not ctx.residual else dres if dres.numel() or not dx.numel() else dx
+    return dx, dw.to(weight.dtype), dres, None, None
+
+
+_fwd.register_autograd(_backward, setup_context=_setup)
+
+
+def _check(name, x, weight, residual):
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{name} needs a feature axis that is not empty")
+    features = x.shape[-1]
+    if weight is not None and weight.shape != (features,):
+        raise ValueError(f"weight must be ({features},), got {tuple(weight.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual must match x {tuple(x.shape)}, got {tuple(residual.shape)}")
+    for label, t in (("x", x), ("weight", weight), ("residual", residual)):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} runs CUDA kernels, {label} is on {t.device}")
+        if t.get_device() != x.get_device():
+            raise ValueError(f"{name}: {label} is on {t.device}, x is on {x.device}")
+        if t.dtype not in _DTYPES:
+            raise ValueError(f"{name} computes float32/bfloat16/float16, {label} is {t.dtype}")
+    if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{name}: the residual stream is {x.dtype} or float32, got {residual.dtype}")
+
+
+def add_rmsnorm(x, weight, residual=None, eps=1e-5):
+    """``stream = x + residual`` and its RMSNorm over the last axis.
+
+    Args:
+        x: ``(..., features)``.
+        weight: ``(features,)``.
+        residual: the residual stream, shaped like ``x``, in x's dtype or
+            float32; None for the first layer.
+        eps: added to the mean square.
+
+    Returns:
+        ``(y, stream)``: y in x's dtype, stream in the residual's (x itself
+        without a residual).
+    """
+    _check("add_rmsnorm", x, weight, residual)
+    if x.numel() == 0:
+        return x.new_empty(x.shape), x if residual is None else x + residual
+    features = x.shape[-1]
+    x2, res2 = _rows(x, features), None if residual is None else _rows(residual, features)
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    if nat.wants_grad(x, weight, residual):
+        y, stream, _ = torch.ops.b200ssm.add_rmsnorm_fwd(x2, w, res2, float(eps), True)
+    elif nat.direct(x2, w, res2):
+        y, stream, _ = _forward(x2, w, res2, float(eps), False)
+    else:
+        y, stream, _ = torch.ops.b200ssm.add_rmsnorm_fwd(x2, w, res2, float(eps), False)
+    return y.view(x.shape), x if residual is None else stream.view(x.shape)
+
+
+def add_rmsnorm_int8(x, weight, residual=None, eps=1e-5):
+    """:func:`add_rmsnorm` with y as int8 rows: ``(q, scale, stream)``, q shaped
+    like ``x``, scale ``x.shape[:-1]`` in float32.  No gradient."""
+    _check("add_rmsnorm_int8", x, weight, residual)
+    if nat.wants_grad(x, weight, residual):
+        raise ValueError("add_rmsnorm_int8 has no gradient: call it under torch.no_grad(), or use add_rmsnorm")
+    if x.numel() == 0:
+        return (x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32),
+                x if residual is None else x + residual)
+    features = x.shape[-1]
+    x2, res2 = _rows(x, features), None if residual is None else _rows(residual, features)
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    fn = _forward_int8 if nat.direct(x2, w, res2) else torch.ops.b200ssm.add_rmsnorm_int8
+    q, scale, stream = fn(x2, w, res2, float(eps))
+    return q.view(x.shape), scale.view(x.shape[:-1]), x if residual is None else stream.view(x.shape)
+
+
+def quantize_int8(x):
+    """The rows of ``x`` (its last axis) as int8 with a float32 scale each:
+    ``(q, scale)``, ``scale = max|x| / 127`` over the row, ``q = rint(x / scale)``.
+    No gradient."""
+    _check("quantize_int8", x, None, None)
+    if nat.wants_grad(x):
+        raise ValueError("quantize_int8 has no gradient: call it under torch.no_grad()")
+    if x.numel() == 0:
+        return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    x2 = _rows(x, x.shape[-1])
+    q, scale = (_quantize if nat.direct(x2) else torch.ops.b200ssm.quantize_int8)(x2)
+    return q.view(x.shape), scale.view(x.shape[:-1])
