@@ -256,21 +256,30 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def stream_here(t: torch.Tensor) -> int:
+    """The current stream's handle on t's device (as :func:`stream_of`, without
+    the 2 us of building a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def direct(*tensors) -> bool:
     """Whether a call without gradients may go to the library itself instead of
     through torch's dispatcher: the tensors are plain ones (no fake or other
     subclass) on the current device, and nothing is being traced.  The
     dispatcher's Python path costs about 15 us a call, more than the kernels
     of a decode step run for."""
-    if torch.compiler.is_compiling():
-        return False
-    plain = (torch.Tensor, torch.nn.Parameter)
-    return (all(t is None or type(t) in plain for t in tensors)
-            and tensors[0].get_device() == torch.cuda.current_device())
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return not torch.compiler.is_compiling() and tensors[0].get_device() == torch._C._cuda_getDevice()
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # --------------------------------------------------------------- status words --

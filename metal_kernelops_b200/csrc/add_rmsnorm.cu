@@ -18,13 +18,14 @@
 //     d  = rstd (w dy - xh c) + dstream,   dx = dresidual = d,   dw = sum_rows dy xh
 //
 // Bytes bound these kernels: each row is read once and kept in registers.  A row
-// belongs to a group of `tx` threads (whole warps; tx NV vectors of 8 elements
-// cover the row), a CTA holds several rows when they are narrow.  The backward
+// belongs to a group of `tx` threads (whole warps; tx NV vectors of V elements
+// cover the row), a CTA holds several rows when they are narrow.  V is 8, or 1
+// where the width or an alignment does not allow 16-byte accesses.  The backward
 // CTAs walk rows blockIdx, blockIdx + grid, ..., keep their columns' dw sums in
 // registers and leave one partial row each; the fold adds the partials in a
-// fixed order, so results are reproducible.  Rows whose width or alignment does
-// not allow 8-element vectors, and rows above 16384 features (8192 in the
-// backward), stream: a CTA reads such a row twice, the second time from L1 / L2.
+// fixed order, so results are reproducible.  Rows wider than the registers of a
+// CTA hold (16384 features forward, 8192 backward) stream: a CTA reads such a row
+// twice, the second time from L1 / L2.
 #include <climits>
 
 #include "common.cuh"
@@ -46,9 +47,16 @@ struct Args {
     int64_t dys, dss;
 };
 
-// Eight consecutive elements.
-template <typename T> struct V8;
-template <> struct V8<float> {
+// V consecutive elements: 8 with vector accesses, or 1.
+template <typename T, int V> struct Vec;
+template <typename T> struct Vec<T, 1> {
+    T r;
+    __device__ __forceinline__ void ld(const T* p) { r = *p; }
+    __device__ __forceinline__ void get(float* v) const { v[0] = ldf(&r); }
+    __device__ __forceinline__ void set(const float* v) { stf(&r, v[0]); }
+    __device__ __forceinline__ void st(T* p) const { *p = r; }
+};
+template <> struct Vec<float, 8> {
     float4 a, b;
     __device__ __forceinline__ void ld(const float* p) {
         a = reinterpret_cast<const float4*>(p)[0];
@@ -66,7 +74,7 @@ template <> struct V8<float> {
         reinterpret_cast<float4*>(p)[1] = b;
     }
 };
-template <typename T, typename H2> struct V8h {
+template <typename T> struct Vec8h {
     uint4 r;
     __device__ __forceinline__ void ld(const T* p) { r = *reinterpret_cast<const uint4*>(p); }
     __device__ __forceinline__ void get(float* v) const {
@@ -85,8 +93,8 @@ template <typename T, typename H2> struct V8h {
     }
     __device__ __forceinline__ void st(T* p) const { *reinterpret_cast<uint4*>(p) = r; }
 };
-template <> struct V8<__nv_bfloat16> : V8h<__nv_bfloat16, __nv_bfloat162> {};
-template <> struct V8<__half> : V8h<__half, __half2> {};
+template <> struct Vec<__nv_bfloat16, 8> : Vec8h<__nv_bfloat16> {};
+template <> struct Vec<__half, 8> : Vec8h<__half> {};
 
 template <typename TS> __device__ __forceinline__ float as_stored(float v);
 template <> __device__ __forceinline__ float as_stored<float>(float v) { return v; }
@@ -95,13 +103,14 @@ template <> __device__ __forceinline__ float as_stored<__nv_bfloat16>(float v) {
 }
 template <> __device__ __forceinline__ float as_stored<__half>(float v) { return __half2float(__float2half_rn(v)); }
 
-__device__ __forceinline__ void ld_weight8(const Args& a, int64_t e, float* w) {
+template <int V>
+__device__ __forceinline__ void ld_weight(const Args& a, int64_t e, float* w) {
     if (a.weight_dtype == SSM_F32) {
-        V8<float> v; v.ld(static_cast<const float*>(a.w) + e); v.get(w);
+        Vec<float, V> v; v.ld(static_cast<const float*>(a.w) + e); v.get(w);
     } else if (a.weight_dtype == SSM_BF16) {
-        V8<__nv_bfloat16> v; v.ld(static_cast<const __nv_bfloat16*>(a.w) + e); v.get(w);
+        Vec<__nv_bfloat16, V> v; v.ld(static_cast<const __nv_bfloat16*>(a.w) + e); v.get(w);
     } else {
-        V8<__half> v; v.ld(static_cast<const __half*>(a.w) + e); v.get(w);
+        Vec<__half, V> v; v.ld(static_cast<const __half*>(a.w) + e); v.get(w);
     }
 }
 
@@ -148,17 +157,24 @@ __device__ __forceinline__ uint32_t pack4(const float* v, float inv) {
     return inv != 0.0f ? __byte_perm(lo, hi, 0x5410) : 0u;
 }
 
-// x (+ residual) -> s, and s stored; the eight s values.
-template <typename T, typename TS>
-__device__ __forceinline__ void sum8(const Args& a, int64_t row, int64_t e, const V8<T>& xr, const V8<TS>& rr,
-                                     float* v) {
+// V int8 values of a row at q.
+template <int V>
+__device__ __forceinline__ void st_q(int8_t* q, const float* v, float inv) {
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(q) = make_uint2(pack4(v, inv), pack4(v + 4, inv));
+    else *q = inv != 0.0f ? (int8_t)(q_bits(v[0], inv) & 0xffu) : (int8_t)0;
+}
+
+// x (+ residual) -> s, and s stored; the V values of s.
+template <typename T, typename TS, int V>
+__device__ __forceinline__ void sum_store(const Args& a, int64_t row, int64_t e, const Vec<T, V>& xr,
+                                          const Vec<TS, V>& rr, float* v) {
     xr.get(v);
     if (a.res != nullptr) {
-        float r[8];
+        float r[V];
         rr.get(r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] + r[i];
-        V8<TS> s;
+        for (int i = 0; i < V; ++i) v[i] = v[i] + r[i];
+        Vec<TS, V> s;
         s.set(v);
         s.get(v);
         s.st(static_cast<TS*>(a.stream) + row * a.features + e);
@@ -167,7 +183,7 @@ __device__ __forceinline__ void sum8(const Args& a, int64_t row, int64_t e, cons
 
 enum Mode { kNorm, kNormInt8, kInt8 };    // y, q and scale, q and scale of x itself
 
-template <typename T, typename TS, int NV, int MODE>
+template <typename T, typename TS, int V, int NV, int MODE>
 __global__ void __launch_bounds__(kMaxThreads)
 fwd_kernel(const Args a) {
     __shared__ SumMax red[kMaxWarps];
@@ -175,12 +191,12 @@ fwd_kernel(const Args a) {
     const int tx = blockDim.x, warps = tx >> 5;
     const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const bool live = row < a.rows;
-    float v[NV][8];
-    V8<T> xr[NV];
-    V8<TS> rr[NV];
+    float v[NV][V];
+    Vec<T, V> xr[NV];
+    Vec<TS, V> rr[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
         if (live && e < F) {
             xr[k].ld(static_cast<const T*>(a.x) + row * a.xs + e);
             if (MODE != kInt8 && a.res != nullptr) rr[k].ld(static_cast<const TS*>(a.res) + row * a.rs + e);
@@ -189,23 +205,23 @@ fwd_kernel(const Args a) {
     SumMax sm{0.0f, 0u};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
         if (live && e < F) {
             if (MODE == kInt8) {
                 xr[k].get(v[k]);
             } else {
-                float w[8];
-                ld_weight8(a, e, w);
-                sum8<T, TS>(a, row, e, xr[k], rr[k], v[k]);
+                float w[V];
+                ld_weight<V>(a, e, w);
+                sum_store<T, TS, V>(a, row, e, xr[k], rr[k], v[k]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < V; ++i) {
                     sm.sum = fmaf(v[k][i], v[k][i], sm.sum);
                     v[k][i] *= w[i];
                 }
             }
             if (MODE != kNorm) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sm.mx = max(sm.mx, abs_bits(v[k][i]));
+                for (int i = 0; i < V; ++i) sm.mx = max(sm.mx, abs_bits(v[k][i]));
             }
         }
     }
@@ -216,11 +232,11 @@ fwd_kernel(const Args a) {
         if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = r;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+            const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
             if (e < F) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[k][i] *= r;
-                V8<T> o;
+                for (int i = 0; i < V; ++i) v[k][i] *= r;
+                Vec<T, V> o;
                 o.set(v[k]);
                 o.st(static_cast<T*>(a.y) + row * F + e);
             }
@@ -230,10 +246,9 @@ fwd_kernel(const Args a) {
         if (threadIdx.x == 0) a.scale[row] = qt.scale1 * r;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+            const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
             if (e < F)
-                *reinterpret_cast<uint2*>(a.q + row * F + e) =
-                    make_uint2(pack4(v[k], qt.inv), pack4(v[k] + 4, qt.inv));
+                st_q<V>(a.q + row * F + e, v[k], qt.inv);
         }
     }
 }
@@ -272,11 +287,11 @@ fwd_stream_kernel(const Args a) {
         float v = MODE == kInt8 ? ldf(x + e) : value(e);
         if (MODE != kInt8) v *= ld_any(a.w, e, a.weight_dtype);
         if (MODE == kNorm) stf(static_cast<T*>(a.y) + row * F + e, v * r);
-        else a.q[row * F + e] = qt.inv != 0.0f ? (int8_t)(q_bits(v, qt.inv) & 0xffu) : (int8_t)0;
+        else st_q<1>(a.q + row * F + e, &v, qt.inv);
     }
 }
 
-template <typename T, typename TS, int NV>
+template <typename T, typename TS, int V, int NV>
 __global__ void __launch_bounds__(kMaxThreads)
 bwd_kernel(const Args a) {
     __shared__ SumMax red[2][kMaxWarps];
@@ -285,26 +300,26 @@ bwd_kernel(const Args a) {
     const TS* s = static_cast<const TS*>(a.stream);
     const T* dy = static_cast<const T*>(a.dy);
     const TS* ds = static_cast<const TS*>(a.ds);
-    float dw[NV][8] = {};
-    float w[NV][8] = {};
+    float dw[NV][V] = {};
+    float w[NV][V] = {};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
-        if (e < F) ld_weight8(a, e, w[k]);
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
+        if (e < F) ld_weight<V>(a, e, w[k]);
     }
     const int64_t step = (int64_t)gridDim.x * blockDim.y;
     int turn = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * blockDim.y; r0 < a.rows; r0 += step, turn ^= 1) {
         const int64_t row = r0 + threadIdx.y;
         const bool live = row < a.rows;
-        V8<TS> sr[NV], dsr[NV];
-        V8<T> dyr[NV];
+        Vec<TS, V> sr[NV], dsr[NV];
+        Vec<T, V> dyr[NV];
         float rstd = 0.0f;
         if (live) {
             rstd = a.rstd[row];
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+                const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
                 if (e < F) {
                     sr[k].ld(s + row * a.xs + e);
                     if (dy) dyr[k].ld(dy + row * a.dys + e);
@@ -313,16 +328,16 @@ bwd_kernel(const Args a) {
             }
         }
         SumMax c{0.0f, 0u};
-        float xh[NV][8], g[NV][8];
+        float xh[NV][V], g[NV][V];
         if (live) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+                const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
                 if (e < F) {
                     sr[k].get(xh[k]);
                     dyr[k].get(g[k]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < V; ++i) {
                         xh[k][i] *= rstd;
                         dw[k][i] = fmaf(g[k][i], xh[k][i], dw[k][i]);
                         g[k][i] *= w[k][i];
@@ -335,17 +350,17 @@ bwd_kernel(const Args a) {
         if (live) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+                const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
                 if (e < F) {
-                    float d[8];
+                    float d[V];
                     if (ds) dsr[k].get(d);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) d[i] = fmaf(rstd, fmaf(-xh[k][i], c1, g[k][i]), ds ? d[i] : 0.0f);
-                    V8<T> o;
+                    for (int i = 0; i < V; ++i) d[i] = fmaf(rstd, fmaf(-xh[k][i], c1, g[k][i]), ds ? d[i] : 0.0f);
+                    Vec<T, V> o;
                     o.set(d);
                     o.st(static_cast<T*>(a.dx) + row * F + e);
                     if (a.dres) {
-                        V8<TS> p;
+                        Vec<TS, V> p;
                         p.set(d);
                         p.st(static_cast<TS*>(a.dres) + row * F + e);
                     }
@@ -357,9 +372,9 @@ bwd_kernel(const Args a) {
     float* part = a.part + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * F;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int64_t e = ((int64_t)k * tx + threadIdx.x) * 8;
+        const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
         if (e < F) {
-            V8<float> o;
+            Vec<float, V> o;
             o.set(dw[k]);
             o.st(part + e);
         }
@@ -420,19 +435,22 @@ __global__ void __launch_bounds__(256) fold_kernel(const float* part, int64_t pa
 static bool al(const void* p, int64_t b) { return (reinterpret_cast<uintptr_t>(p) % b) == 0; }
 static int64_t esize(int dtype) { return dtype == SSM_F32 ? 4 : 2; }
 
-// The widest rows that a CTA's registers hold: 512 threads x 32 elements in the
-// forward; x 16 in the backward, which also keeps the weights and their sums.
-constexpr int64_t kMaxFwd = kMaxThreads * 32, kMaxBwd = kMaxThreads * 16;
-
-// nv = 0: the streaming kernels.
-struct Shape { int tx, ty, nv; };
+// v elements a vector (8, or 1 where width or alignment does not allow 8), nv
+// vectors a thread, tx threads a row, ty rows a CTA; nv = 0: the streaming
+// kernels.  Rows of up to 512 vectors take one vector a thread (v = 8).
+struct Shape { int tx, ty, v, nv; };
 
 static Shape shape_of(int64_t F, bool vec, bool bwd) {
-    if (!vec || F > (bwd ? kMaxBwd : kMaxFwd)) return {(int)min64(kMaxThreads, ceil_div(F, 32) * 32), 1, 0};
-    const int64_t n = F / 8;
-    const int nv = n <= 512 ? 1 : n <= 1024 ? 2 : 4;
+    const int v = vec ? 8 : 1;
+    const int64_t n = ceil_div(F, v);
+    int nv = 0;
+    for (int c : {1, 2, 4})
+        if (vec && nv == 0 && n <= (int64_t)c * kMaxThreads && !(bwd && c == 4)) nv = c;
+    for (int c : {8, 16})
+        if (!vec && nv == 0 && n <= (int64_t)c * kMaxThreads) nv = c;
+    if (nv == 0) return {kMaxThreads, 1, 1, 0};
     const int tx = (int)(ceil_div(ceil_div(n, nv), 32) * 32);
-    return {tx, tx >= 128 ? 1 : 128 / tx, nv};
+    return {tx, tx >= 128 ? 1 : 128 / tx, v, nv};
 }
 
 static int validate(const ssm_add_rmsnorm_params* p, const char* op) {
@@ -471,9 +489,11 @@ static int launch_fwd(const Args& a, const Shape& s, cudaStream_t st) {
     const unsigned grid = (unsigned)ceil_div(a.rows, s.ty);
     switch (s.nv) {
         case 0: fwd_stream_kernel<T, TS, MODE><<<grid, block, 0, st>>>(a); break;
-        case 1: fwd_kernel<T, TS, 1, MODE><<<grid, block, 0, st>>>(a); break;
-        case 2: fwd_kernel<T, TS, 2, MODE><<<grid, block, 0, st>>>(a); break;
-        default: fwd_kernel<T, TS, 4, MODE><<<grid, block, 0, st>>>(a);
+        case 1: fwd_kernel<T, TS, 8, 1, MODE><<<grid, block, 0, st>>>(a); break;
+        case 2: fwd_kernel<T, TS, 8, 2, MODE><<<grid, block, 0, st>>>(a); break;
+        case 4: fwd_kernel<T, TS, 8, 4, MODE><<<grid, block, 0, st>>>(a); break;
+        case 8: fwd_kernel<T, TS, 1, 8, MODE><<<grid, block, 0, st>>>(a); break;
+        default: fwd_kernel<T, TS, 1, 16, MODE><<<grid, block, 0, st>>>(a);
     }
     return check_launch(MODE == kInt8 ? "quantize_int8" : "add_rmsnorm fwd");
 }
@@ -506,8 +526,10 @@ static void launch_bwd(const Args& a, const Shape& s, int64_t ctas, cudaStream_t
     const dim3 block(s.tx, s.ty);
     switch (s.nv) {
         case 0: bwd_stream_kernel<T, TS><<<(unsigned)ctas, block, 0, st>>>(a); break;
-        case 1: bwd_kernel<T, TS, 1><<<(unsigned)ctas, block, 0, st>>>(a); break;
-        default: bwd_kernel<T, TS, 2><<<(unsigned)ctas, block, 0, st>>>(a);
+        case 1: bwd_kernel<T, TS, 8, 1><<<(unsigned)ctas, block, 0, st>>>(a); break;
+        case 2: bwd_kernel<T, TS, 8, 2><<<(unsigned)ctas, block, 0, st>>>(a); break;
+        case 8: bwd_kernel<T, TS, 1, 8><<<(unsigned)ctas, block, 0, st>>>(a); break;
+        default: bwd_kernel<T, TS, 1, 16><<<(unsigned)ctas, block, 0, st>>>(a);
     }
 }
 
@@ -519,9 +541,12 @@ using namespace ssm::anorm;
 
 extern "C" int ssm_add_rmsnorm_sizes(const ssm_add_rmsnorm_params* p, size_t* workspace_bytes) {
     if (int s = validate(p, "add_rmsnorm")) return s;
-    // either kernel's partial rows (the vector kernels leave one per row group)
-    const Shape sh = shape_of(p->features, p->features % 8 == 0, true);
-    const int64_t parts = max64(bwd_ctas(p->rows, sh.ty) * sh.ty, bwd_ctas(p->rows, 1));
+    // the partial rows of either form (the pointers' alignment picks one): a CTA leaves one per row group
+    int64_t parts = 0;
+    for (bool vec : {false, true}) {
+        const Shape sh = shape_of(p->features, vec && p->features % 8 == 0, true);
+        parts = max64(parts, bwd_ctas(p->rows, sh.ty) * sh.ty);
+    }
     if (workspace_bytes) *workspace_bytes = (size_t)(parts * p->features) * 4;
     return SSM_OK;
 }

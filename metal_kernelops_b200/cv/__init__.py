@@ -18,12 +18,12 @@ The reference's other ``cv`` families (NSA selection, RoIAlign) are outside
 this package's scope.
 """
 
-from .add_rmsnorm import add_rmsnorm, add_rmsnorm_int8, quantize_int8
 from .causal_conv1d import causal_conv1d_fn, causal_conv1d_update
 from .gated_norm import rmsnorm_gated
 from .mamba2_chunk import last_path, mamba2_chunk_scan, tc_shape
 from .mamba2_state import mamba2_state_update
 from .path_scan import path_orders, ss2d_scan
+from .residual_norm import add_rmsnorm, add_rmsnorm_int8, quantize_int8
 
 __all__ = ["add_rmsnorm", "add_rmsnorm_int8", "quantize_int8", "causal_conv1d_fn", "causal_conv1d_update", "last_path", "mamba2_chunk_scan",
            "mamba2_state_update", "path_orders", "rmsnorm_gated", "ss2d_scan", "tc_shape"]

@@ -46,46 +46,63 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _features(t):
+    """t itself when its rows are contiguous features with even spacing (any
+    leading shape if t is contiguous, else two axes), a two-axis view or a copy
+    otherwise."""
+    return t if t.is_contiguous() else _rows(t, t.shape[-1])
+
+
 def _params(x, residual, weight, eps, stream=None, y=None, q=None, scale=None, rstd=None):
-    stream_dtype = x.dtype if residual is None else residual.dtype
+    features = x.shape[-1]
+    code = nat.dtype_code(x.dtype)
     return nat.AddRmsNormParams(
-        x.shape[0], x.shape[1], _stride(x), _stride(residual), 0, 0, nat.dtype_code(x.dtype),
-        nat.dtype_code(stream_dtype), 0 if weight is None else nat.dtype_code(weight.dtype), eps, x.data_ptr(),
+        x.numel() // features, features, 0 if x.is_contiguous() else _stride(x),
+        0 if residual is None or residual.is_contiguous() else _stride(residual), 0, 0, code,
+        code if residual is None else nat.dtype_code(residual.dtype),
+        0 if weight is None else nat.dtype_code(weight.dtype), eps, x.data_ptr(),
         _ptr(residual), _ptr(weight), _ptr(stream), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
 
 
-def _forward(x, weight, residual, eps, save):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stream = torch.empty(x.shape if residual is not None else (0,),
-                         dtype=x.dtype if residual is None else residual.dtype, device=x.device)
-    rstd = torch.empty(x.shape[0] if save else 0, dtype=torch.float32, device=x.device)
-    p = _params(x, residual, weight, eps, stream if residual is not None else None, y, rstd=rstd if save else None)
-    nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_of(x)), "add_rmsnorm")
+# The launches.  `shape` is the outputs' shape; x and residual are its rows.
+def _forward(x, weight, residual, eps, save, shape):
+    dev = x.device
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    stream = None if residual is None else torch.empty(shape, dtype=residual.dtype, device=dev)
+    rstd = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if save else None
+    p = _params(x, residual, weight, eps, stream, y, rstd=rstd)
+    nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_here(x)), "add_rmsnorm")
     return y, stream, rstd
 
 
-def _forward_int8(x, weight, residual, eps):
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-    stream = torch.empty(x.shape if residual is not None else (0,),
-                         dtype=x.dtype if residual is None else residual.dtype, device=x.device)
-    p = _params(x, residual, weight, eps, stream if residual is not None else None, q=q, scale=scale)
-    nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_of(x)), "add_rmsnorm_int8")
+def _forward_int8(x, weight, residual, eps, shape):
+    dev = x.device
+    q = torch.empty(shape, dtype=torch.int8, device=dev)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    stream = None if residual is None else torch.empty(shape, dtype=residual.dtype, device=dev)
+    p = _params(x, residual, weight, eps, stream, q=q, scale=scale)
+    nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_here(x)), "add_rmsnorm_int8")
     return q, scale, stream
 
 
-def _quantize(x):
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-    p = _params(x, None, None, 0.0, q=q, scale=scale)
-    nat.check(nat.lib().ssm_quantize_int8(p, nat.stream_of(x)), "quantize_int8")
+def _quantize(x, shape):
+    q = torch.empty(shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    nat.check(nat.lib().ssm_quantize_int8(_params(x, None, None, 0.0, q=q, scale=scale), nat.stream_here(x)),
+              "quantize_int8")
     return q, scale
+
+
+def _none_empty(t, like, dtype):
+    """Custom ops return tensors: an empty one in the place of an absent output."""
+    return torch.empty(0, dtype=dtype, device=like.device) if t is None else t
 
 
 @torch.library.custom_op("b200ssm::add_rmsnorm_fwd", mutates_args=(), device_types="cuda")
 def _fwd(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor], eps: float,
          save: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _forward(x, weight, residual, eps, save)
+    y, stream, rstd = _forward(x, weight, residual, eps, save, x.shape)
+    return y, _none_empty(stream, x, x.dtype), _none_empty(rstd, x, torch.float32)
 
 
 @_fwd.register_fake
@@ -97,7 +114,8 @@ def _(x, weight, residual, eps, save):
 @torch.library.custom_op("b200ssm::add_rmsnorm_int8", mutates_args=(), device_types="cuda")
 def _int8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor],
           eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _forward_int8(x, weight, residual, eps)
+    q, scale, stream = _forward_int8(x, weight, residual, eps, x.shape)
+    return q, scale, _none_empty(stream, x, x.dtype)
 
 
 @_int8.register_fake
@@ -108,7 +126,7 @@ def _(x, weight, residual, eps):
 
 @torch.library.custom_op("b200ssm::quantize_int8", mutates_args=(), device_types="cuda")
 def _quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return _quantize(x)
+    return _quantize(x, x.shape)
 
 
 @_quant.register_fake
@@ -168,23 +186,24 @@ _fwd.register_autograd(_backward, setup_context=_setup)
 
 
 def _check(name, x, weight, residual):
-    if x.dim() < 1 or x.shape[-1] == 0:
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError(f"{name} needs a feature axis that is not empty")
-    features = x.shape[-1]
-    if weight is not None and weight.shape != (features,):
-        raise ValueError(f"weight must be ({features},), got {tuple(weight.shape)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual must match x {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if weight is not None and weight.shape != shape[-1:]:
+        raise ValueError(f"weight must be ({shape[-1]},), got {tuple(weight.shape)}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must match x {tuple(shape)}, got {tuple(residual.shape)}")
+    index = x.get_device()
     for label, t in (("x", x), ("weight", weight), ("residual", residual)):
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError(f"{name} runs CUDA kernels, {label} is on {t.device}")
-        if t.get_device() != x.get_device():
+        if t.get_device() != index:
             raise ValueError(f"{name}: {label} is on {t.device}, x is on {x.device}")
         if t.dtype not in _DTYPES:
             raise ValueError(f"{name} computes float32/bfloat16/float16, {label} is {t.dtype}")
-    if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+    if residual is not None and residual.dtype is not x.dtype and residual.dtype is not torch.float32:
         raise ValueError(f"{name}: the residual stream is {x.dtype} or float32, got {residual.dtype}")
 
 
@@ -205,15 +224,15 @@ def add_rmsnorm(x, weight, residual=None, eps=1e-5):
     _check("add_rmsnorm", x, weight, residual)
     if x.numel() == 0:
         return x.new_empty(x.shape), x if residual is None else x + residual
-    features = x.shape[-1]
-    x2, res2 = _rows(x, features), None if residual is None else _rows(residual, features)
     w = weight if weight.is_contiguous() else weight.contiguous()
-    if nat.wants_grad(x, weight, residual):
-        y, stream, _ = torch.ops.b200ssm.add_rmsnorm_fwd(x2, w, res2, float(eps), True)
-    elif nat.direct(x2, w, res2):
-        y, stream, _ = _forward(x2, w, res2, float(eps), False)
-    else:
-        y, stream, _ = torch.ops.b200ssm.add_rmsnorm_fwd(x2, w, res2, float(eps), False)
+    if not nat.wants_grad(x, weight, residual) and nat.direct(x, w, residual):
+        y, stream, _ = _forward(_features(x), w, None if residual is None else _features(residual), float(eps),
+                                False, x.shape)
+        return y, x if residual is None else stream
+    features = x.shape[-1]
+    y, stream, _ = torch.ops.b200ssm.add_rmsnorm_fwd(
+        _rows(x, features), w, None if residual is None else _rows(residual, features), float(eps),
+        nat.wants_grad(x, weight, residual))
     return y.view(x.shape), x if residual is None else stream.view(x.shape)
 
 
@@ -226,11 +245,14 @@ def add_rmsnorm_int8(x, weight, residual=None, eps=1e-5):
     if x.numel() == 0:
         return (x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32),
                 x if residual is None else x + residual)
-    features = x.shape[-1]
-    x2, res2 = _rows(x, features), None if residual is None else _rows(residual, features)
     w = weight if weight.is_contiguous() else weight.contiguous()
-    fn = _forward_int8 if nat.direct(x2, w, res2) else torch.ops.b200ssm.add_rmsnorm_int8
-    q, scale, stream = fn(x2, w, res2, float(eps))
+    if nat.direct(x, w, residual):
+        q, scale, stream = _forward_int8(_features(x), w, None if residual is None else _features(residual),
+                                         float(eps), x.shape)
+        return q, scale, x if residual is None else stream
+    features = x.shape[-1]
+    q, scale, stream = torch.ops.b200ssm.add_rmsnorm_int8(
+        _rows(x, features), w, None if residual is None else _rows(residual, features), float(eps))
     return q.view(x.shape), scale.view(x.shape[:-1]), x if residual is None else stream.view(x.shape)
 
 
@@ -243,6 +265,7 @@ def quantize_int8(x):
         raise ValueError("quantize_int8 has no gradient: call it under torch.no_grad()")
     if x.numel() == 0:
         return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
-    x2 = _rows(x, x.shape[-1])
-    q, scale = (_quantize if nat.direct(x2) else torch.ops.b200ssm.quantize_int8)(x2)
+    if nat.direct(x):
+        return _quantize(_features(x), x.shape)
+    q, scale = torch.ops.b200ssm.quantize_int8(_rows(x, x.shape[-1]))
     return q.view(x.shape), scale.view(x.shape[:-1])
