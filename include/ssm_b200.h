@@ -532,6 +532,84 @@ int ssm_add_rmsnorm_fwd(const ssm_add_rmsnorm_params* p, void* stream);
 int ssm_add_rmsnorm_bwd(const ssm_add_rmsnorm_params* p, void* stream);
 int ssm_quantize_int8(const ssm_add_rmsnorm_params* p, void* stream);
 
+/* ------------------------------------------------------------------------- *
+ * Gated linear recurrence: one state per channel, a forget gate per token.  No
+ * counterpart in the reference.
+ *
+ *     g_t = (1 - lower) sigmoid(-forget_t)
+ *     h_t = (1 - g_t) h'_t + g_t x_t,   h'_t = 0 where reset_t, else h_{t-1}
+ *     y_t = h_t silu(z_t)               (h_t without z)
+ *
+ *   x, forget, z, y, dy, dx, dforget, dz : (batch, length, dim), dtype
+ *   lower, dlower (dim): fp32, lower in [0, 1), NULL: 0
+ *   initial_state, final_state, dfinal, dinitial : (batch, dim) fp32
+ *                                         (initial_state NULL: zeros)
+ *   reset : (batch, length) bytes, non-zero where a sequence begins (NULL: none)
+ *   states : fp32, states_bytes of ssm_gated_recurrence_sizes, written by the
+ *            forward (NULL: not saved) and read by the backward
+ * z, dfinal, dinitial and dlower may be NULL.  The backward takes a workspace of
+ * workspace_bytes.  A state that is not finite does not pass a reset.
+ * ------------------------------------------------------------------------- */
+typedef struct ssm_gated_recurrence_params {
+    int64_t batch, length, dim;
+    /* elements between tokens (0: dim) and between batch rows (0: length
+     * tokens); channels are contiguous.  y, dx, dforget and dz are dense. */
+    int64_t x_token_stride, x_batch_stride, forget_token_stride, forget_batch_stride;
+    int64_t z_token_stride, z_batch_stride, dy_token_stride, dy_batch_stride;
+    int32_t dtype;
+    uint32_t flags;             /* none defined */
+    const void* x;
+    const void* forget;
+    const void* z;
+    const float* lower;
+    const float* initial_state;
+    const uint8_t* reset;
+    void* y;
+    float* final_state;
+    float* states;
+    const void* dy;
+    const float* dfinal;
+    void* dx;
+    void* dforget;
+    void* dz;
+    float* dlower;
+    float* dinitial;
+    void* workspace;
+    size_t workspace_bytes;
+    /* optional device word (NULL: none).  A kernel of this op that gives up
+     * on a bounded wait writes its non-zero code here (the first failure
+     * wins; the word is never cleared by the library), besides the per-device
+     * flag that ssm_take_kernel_error reads.  Start it at 0. */
+    int32_t* status;
+} ssm_gated_recurrence_params;
+
+int ssm_gated_recurrence_sizes(const ssm_gated_recurrence_params* p, size_t* states_bytes,
+                               size_t* workspace_bytes);
+int ssm_gated_recurrence_fwd(const ssm_gated_recurrence_params* p, void* stream);
+int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, void* stream);
+
+/* One token per row: `state` (batch, dim) fp32 is updated in place.  x, forget,
+ * z and y are (batch, dim) in dtype, y dense; the batch strides (0: dim) let
+ * the others be slices of wider buffers. */
+typedef struct ssm_gated_recurrence_step_params {
+    int64_t batch, dim;
+    int64_t x_batch_stride, forget_batch_stride, z_batch_stride, state_batch_stride;
+    int32_t dtype;
+    uint32_t flags;             /* none defined */
+    const void* x;
+    const void* forget;
+    const void* z;
+    const float* lower;
+    float* state;
+    void* y;
+    /* optional device word (NULL: none), the same slot every op's params
+     * carry; this op's kernels have no waits that can give up and never
+     * write it. */
+    int32_t* status;
+} ssm_gated_recurrence_step_params;
+
+int ssm_gated_recurrence_step(const ssm_gated_recurrence_step_params* p, void* stream);
+
 /* Kernels that wait on an mbarrier give up after a bounded number of polls,
  * record a non-zero code in a per-device flag (and in the call's `status`
  * word, when given) and return.  This reads the flag of the current device

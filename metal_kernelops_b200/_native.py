@@ -48,6 +48,8 @@ EXPORTS = (
     "ssm_causal_conv1d_update",
     "ssm_gated_rmsnorm_sizes", "ssm_gated_rmsnorm_fwd", "ssm_gated_rmsnorm_bwd",
     "ssm_add_rmsnorm_sizes", "ssm_add_rmsnorm_fwd", "ssm_add_rmsnorm_bwd", "ssm_quantize_int8",
+    "ssm_gated_recurrence_sizes", "ssm_gated_recurrence_fwd", "ssm_gated_recurrence_bwd",
+    "ssm_gated_recurrence_step",
 )
 
 _I64, _I32, _U32, _P, _SZ = ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t
@@ -161,6 +163,33 @@ class AddRmsNormParams(ctypes.Structure):
     ]
 
 
+class GatedRecurrenceParams(ctypes.Structure):
+    _fields_ = [
+        ("batch", _I64), ("length", _I64), ("dim", _I64),
+        ("x_token_stride", _I64), ("x_batch_stride", _I64),
+        ("forget_token_stride", _I64), ("forget_batch_stride", _I64),
+        ("z_token_stride", _I64), ("z_batch_stride", _I64),
+        ("dy_token_stride", _I64), ("dy_batch_stride", _I64),
+        ("dtype", _I32), ("flags", _U32),
+        ("x", _P), ("forget", _P), ("z", _P), ("lower", _P), ("initial_state", _P), ("reset", _P),
+        ("y", _P), ("final_state", _P), ("states", _P),
+        ("dy", _P), ("dfinal", _P), ("dx", _P), ("dforget", _P), ("dz", _P), ("dlower", _P), ("dinitial", _P),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+        ("status", _P),
+    ]
+
+
+class GatedRecurrenceStepParams(ctypes.Structure):
+    _fields_ = [
+        ("batch", _I64), ("dim", _I64),
+        ("x_batch_stride", _I64), ("forget_batch_stride", _I64), ("z_batch_stride", _I64),
+        ("state_batch_stride", _I64),
+        ("dtype", _I32), ("flags", _U32),
+        ("x", _P), ("forget", _P), ("z", _P), ("lower", _P), ("state", _P), ("y", _P),
+        ("status", _P),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -187,7 +216,8 @@ def lib():
                                  ("ss2d_scan", Ss2dScanParams),
                                  ("causal_conv1d", CausalConv1dParams),
                                  ("gated_rmsnorm", GatedRmsNormParams),
-                                 ("add_rmsnorm", AddRmsNormParams)):
+                                 ("add_rmsnorm", AddRmsNormParams),
+                                 ("gated_recurrence", GatedRecurrenceParams)):
                 for suffix in ("fwd", "bwd"):
                     fn = getattr(handle, f"ssm_{name}_{suffix}")
                     fn.restype = ctypes.c_int
@@ -201,6 +231,11 @@ def lib():
             handle.ssm_causal_conv1d_sizes.argtypes = [ctypes.POINTER(CausalConv1dParams), ctypes.POINTER(_SZ)]
             handle.ssm_gated_rmsnorm_sizes.argtypes = [ctypes.POINTER(GatedRmsNormParams), ctypes.POINTER(_SZ)]
             handle.ssm_add_rmsnorm_sizes.argtypes = [ctypes.POINTER(AddRmsNormParams), ctypes.POINTER(_SZ)]
+            handle.ssm_gated_recurrence_sizes.argtypes = [
+                ctypes.POINTER(GatedRecurrenceParams), ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]
+            handle.ssm_gated_recurrence_step.restype = ctypes.c_int
+            handle.ssm_gated_recurrence_step.argtypes = [ctypes.POINTER(GatedRecurrenceStepParams),
+                                                         ctypes.c_void_p]
             handle.ssm_quantize_int8.restype = ctypes.c_int
             handle.ssm_quantize_int8.argtypes = [ctypes.POINTER(AddRmsNormParams), ctypes.c_void_p]
             handle.ssm_causal_conv1d_update.restype = ctypes.c_int
@@ -215,7 +250,8 @@ def lib():
                                                             ctypes.c_void_p]
             for name in ("ssm_selective_scan_sizes", "ssm_state_update_sizes", "ssm_chunk_scan_sizes",
                          "ssm_ss2d_scan_sizes", "ssm_selective_scan_fwd_workspace",
-                         "ssm_causal_conv1d_sizes", "ssm_gated_rmsnorm_sizes", "ssm_add_rmsnorm_sizes"):
+                         "ssm_causal_conv1d_sizes", "ssm_gated_rmsnorm_sizes", "ssm_add_rmsnorm_sizes",
+                         "ssm_gated_recurrence_sizes"):
                 getattr(handle, name).restype = ctypes.c_int
             handle.ssm_take_kernel_error.restype = ctypes.c_int
             handle.ssm_take_kernel_error.argtypes = []

@@ -1,0 +1,511 @@
+// Gated linear recurrence for sm_100a: a diagonal recurrence with one state per
+// channel whose forget gate comes with every token; forward over sequences, its
+// backward pass, and the single-token step.
+//
+// Per batch row and channel, with span = 1 - lower (the channel's lower bound of
+// the forget gate), all in fp32:
+//     k_t = sigmoid(-forget_t),   g_t = span k_t
+//     h'_t = 0 where reset_t, else h_{t-1}
+//     h_t = g_t x_t + (h'_t - g_t h'_t)      (two fused steps; exactly x_t where g_t = 1)
+//     y_t = h_t silu(z_t)                    (h_t without z)
+// k_t is 1 / (1 + e^forget): the complement of the gate is computed as such, so
+// that gates near one (long memory) keep their full relative precision.
+// Backward, with dh_t the gradient of h_t and a_t = 1 - g_t (0 at a reset):
+//     dh_t = dy_t silu(z_t) + a_{t+1} dh_{t+1}   (+ dfinal at the last step)
+//     dx = g dh,  dg = dh (x - h'),  dforget = -dg g (1 - k),  dlower = -sum dg k
+//     dz = dy h silu'(z),  dinitial = a_0 dh_0
+//
+// Both directions are scans of affine maps: a run of steps takes the state S to
+// A S + H, with A the product of the a_t, and the gradient D that enters it from
+// the later steps to A D + R.  A warp owns kSteps consecutive steps of a tile of
+// channels (a lane: one 4-byte word, two 16-bit channels or one fp32 channel),
+// holds them in registers, and reduces them to (A, H); the warps' maps meet in
+// shared memory, each warp composes those before it and walks its steps a second
+// time from the right start.  A CTA's kWarps warps make a chunk, and the CTA goes
+// through the chunks of its rows in order.
+// A composition whose A is exactly 0 (a reset) takes H alone: a state that is not
+// finite does not pass a reset.
+// The forward saves the state that enters each chunk, in fp32, for the backward,
+// which recomputes the chunk's states from it.
+#include <climits>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace ssm {
+namespace glr {
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kSteps = 8, kChunk = kWarps * kSteps;
+
+struct Args {
+    int64_t batch, length, dim, chunks;
+    int64_t xt, xb, ft, fb, zt, zb, dyt, dyb;      // token and batch strides
+    const void* x; const void* forget; const void* z;
+    const float* lower; const float* init; const uint8_t* reset;
+    void* y; float* final_state; float* states;
+    const void* dy; const float* dfinal;
+    void* dx; void* dforget; void* dz; float* dinit; float* part;
+    int words;                                      // 4-byte accesses are aligned
+};
+
+// ------------------------------------------------- one or two channels a lane --
+template <typename T> struct Lane { using F = float2; static constexpr int E = 2; };
+template <> struct Lane<float> { using F = float; static constexpr int E = 1; };
+
+__device__ __forceinline__ float fm(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 fm(float2 a, float2 b, float2 c) { return fma2(a, b, c); }
+__device__ __forceinline__ float mu(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 mu(float2 a, float2 b) { return mul2(a, b); }
+__device__ __forceinline__ float ad(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 ad(float2 a, float2 b) { return add2(a, b); }
+template <typename F> __device__ __forceinline__ F same(float v);
+template <> __device__ __forceinline__ float same<float>(float v) { return v; }
+template <> __device__ __forceinline__ float2 same<float2>(float v) { return f2(v); }
+template <typename F> __device__ __forceinline__ F sub(F a, F b) { return fm(b, same<F>(-1.0f), a); }
+template <typename F> __device__ __forceinline__ F neg(F a) { return mu(a, same<F>(-1.0f)); }
+template <typename F> __device__ __forceinline__ F step(F h, F g, F x) { return fm(g, x, fm(neg(g), h, h)); }
+
+// 2^v, with v limited to 120 so that 1 + 2^v stays finite (NaN passes).
+__device__ __forceinline__ float ex2_limited(float v) {
+    float m;
+    asm("min.NaN.f32 %0, %1, 0f42F00000;" : "=f"(m) : "f"(v));
+    return exp2_mufu(m);
+}
+// 1 / (1 + e^v): two MUFU operations.
+__device__ __forceinline__ float sigmoid_neg(float v) { return rcp_mufu(1.0f + ex2_limited(v * kLog2e)); }
+__device__ __forceinline__ float2 sigmoid_neg(float2 v) {
+    const float2 m = mul2(v, f2(kLog2e));
+    const float2 d = add2(f2(1.0f), make_float2(ex2_limited(m.x), ex2_limited(m.y)));
+    return make_float2(rcp_mufu(d.x), rcp_mufu(d.y));
+}
+
+// S -> A S + H; where A is 0 the state that enters does not matter.
+__device__ __forceinline__ float through(float A, float H, float S) { return A == 0.0f ? H : fmaf(A, S, H); }
+__device__ __forceinline__ float2 through(float2 A, float2 H, float2 S) {
+    return make_float2(through(A.x, H.x, S.x), through(A.y, H.y, S.y));
+}
+
+template <typename T> __device__ __forceinline__ typename Lane<T>::F unpack(uint32_t w);
+template <> __device__ __forceinline__ float unpack<float>(uint32_t w) { return __uint_as_float(w); }
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// The lane's word at p: channels c (and c + 1) of `dim`; zero outside.
+template <typename T>
+__device__ __forceinline__ uint32_t ld_word(const T* p, int64_t c, int64_t dim, bool words) {
+    if constexpr (sizeof(T) == 4) {
+        return c < dim ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+    } else {
+        if (words && c + 1 < dim) return *reinterpret_cast<const uint32_t*>(p);
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+        uint32_t w = c < dim ? h[0] : 0u;
+        if (c + 1 < dim) w |= (uint32_t)h[1] << 16;
+        return w;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void st_word(T* p, typename Lane<T>::F v, int64_t c, int64_t dim, bool words) {
+    if constexpr (sizeof(T) == 4) {
+        if (c < dim) *p = v;
+    } else {
+        if (words && c + 1 < dim) {
+            Io2<T>::st(p, v);
+        } else {
+            if (c < dim) stf(p, v.x);
+            if (c + 1 < dim) stf(p + 1, v.y);
+        }
+    }
+}
+// The lane's channels of a per-channel fp32 array; `none` where absent or outside.
+__device__ __forceinline__ void ld_chan(const float* p, int64_t c, int64_t dim, float none, float& v) {
+    v = (p != nullptr && c < dim) ? p[c] : none;
+}
+__device__ __forceinline__ void ld_chan(const float* p, int64_t c, int64_t dim, float none, float2& v) {
+    v.x = (p != nullptr && c < dim) ? p[c] : none;
+    v.y = (p != nullptr && c + 1 < dim) ? p[c + 1] : none;
+}
+__device__ __forceinline__ void st_chan(float* p, int64_t c, int64_t dim, float v) {
+    if (c < dim) p[c] = v;
+}
+__device__ __forceinline__ void st_chan(float* p, int64_t c, int64_t dim, float2 v) {
+    if (c < dim) p[c] = v.x;
+    if (c + 1 < dim) p[c + 1] = v.y;
+}
+
+// Bit i: the i-th of the warp's steps (from t) is a reset.
+__device__ __forceinline__ uint32_t reset_mask(const uint8_t* reset, int64_t row, int64_t t, int64_t length) {
+    if (reset == nullptr) return 0u;
+    const int lane = threadIdx.x & 31;
+    const bool r = lane < kSteps && t + lane < length && reset[row + t + lane] != 0;
+    return __ballot_sync(0xffffffffu, r);
+}
+
+template <typename T>
+__device__ __forceinline__ void ld_steps(const void* base, int64_t row, int64_t stride, int64_t t, int n, int64_t c,
+                                         const Args& a, uint32_t* w) {
+    const T* p = static_cast<const T*>(base) + row + t * stride + c;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) w[i] = i < n ? ld_word<T>(p + i * stride, c, a.dim, a.words) : 0u;
+}
+
+template <typename F> struct Map { F A, H; };
+
+template <typename T, bool GATE>
+__global__ void __launch_bounds__(kThreads)
+fwd_kernel(const Args a) {
+    using F = typename Lane<T>::F;
+    constexpr int E = Lane<T>::E;
+    __shared__ Map<F> maps[2][kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t b = blockIdx.y, c = ((int64_t)blockIdx.x * 32 + lane) * E;
+    F span, S;
+    ld_chan(a.lower, c, a.dim, 0.0f, span);
+    span = sub(same<F>(1.0f), span);
+    ld_chan(a.init ? a.init + b * a.dim : nullptr, c, a.dim, 0.0f, S);
+    for (int64_t n = 0; n < a.chunks; ++n) {
+        const int64_t t = n * kChunk + warp * kSteps;
+        const int live = (int)max64(0, min64(kSteps, a.length - t));
+        uint32_t xw[kSteps], fw[kSteps], zw[kSteps];
+        ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
+        ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
+        if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
+        const uint32_t rs = reset_mask(a.reset, b * a.length, t, a.length);
+        F g[kSteps];
+        Map<F> m{same<F>(1.0f), same<F>(0.0f)};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            g[i] = i < live ? mu(span, sigmoid_neg(unpack<T>(fw[i]))) : same<F>(0.0f);
+            if (rs >> i & 1u) m = {same<F>(0.0f), same<F>(0.0f)};
+            m.H = step(m.H, g[i], unpack<T>(xw[i]));
+            m.A = fm(m.A, neg(g[i]), m.A);
+        }
+        Map<F>(*mw)[32] = maps[n & 1];
+        mw[warp][lane] = m;
+        __syncthreads();
+        if (a.states != nullptr && warp == 0)
+            st_chan(a.states + (b * a.chunks + n) * a.dim, c, a.dim, S);
+        F h = S;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const Map<F> o = mw[w][lane];
+            if (w == warp) h = S;
+            S = through(o.A, o.H, S);
+        }
+        T* y = static_cast<T*>(a.y) + (b * a.length + t) * a.dim + c;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (rs >> i & 1u) h = same<F>(0.0f);
+            h = step(h, g[i], unpack<T>(xw[i]));
+            F o = h;
+            if (GATE) {
+                const F z = unpack<T>(zw[i]);
+                o = mu(h, mu(z, sigmoid_neg(neg(z))));
+            }
+            if (i < live) st_word<T>(y + i * a.dim, o, c, a.dim, a.words);
+        }
+    }
+    if (warp == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
+}
+
+template <typename T, bool GATE>
+__global__ void __launch_bounds__(kThreads)
+bwd_kernel(const Args a) {
+    using F = typename Lane<T>::F;
+    constexpr int E = Lane<T>::E;
+    __shared__ struct { Map<F> m[32]; F R[32]; } maps[2][kWarps];
+    __shared__ F sums[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t b = blockIdx.y, c = ((int64_t)blockIdx.x * 32 + lane) * E;
+    const F one = same<F>(1.0f), zero = same<F>(0.0f);
+    F span, D;
+    ld_chan(a.lower, c, a.dim, 0.0f, span);
+    span = sub(one, span);
+    ld_chan(a.dfinal ? a.dfinal + b * a.dim : nullptr, c, a.dim, 0.0f, D);
+    F dlower = zero;
+    for (int64_t n = a.chunks - 1; n >= 0; --n) {
+        const int64_t t = n * kChunk + warp * kSteps;
+        const int live = (int)max64(0, min64(kSteps, a.length - t));
+        uint32_t xw[kSteps], fw[kSteps], zw[kSteps], dw[kSteps];
+        ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
+        ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
+        if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
+        ld_steps<T>(a.dy, b * a.dyb, a.dyt, t, live, c, a, dw);
+        F h;
+        ld_chan(a.states + (b * a.chunks + n) * a.dim, c, a.dim, 0.0f, h);
+        const uint32_t rs = reset_mask(a.reset, b * a.length, t, a.length);
+        F k[kSteps];
+        Map<F> m{one, zero};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            k[i] = i < live ? sigmoid_neg(unpack<T>(fw[i])) : zero;
+            const F g = mu(span, k[i]);
+            if (rs >> i & 1u) m = {zero, zero};
+            m.H = step(m.H, g, unpack<T>(xw[i]));
+            m.A = fm(m.A, neg(g), m.A);
+        }
+        F d = zero;
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i) {
+            F e = unpack<T>(dw[i]);
+            if (GATE) {
+                const F z = unpack<T>(zw[i]);
+                e = mu(e, mu(z, sigmoid_neg(neg(z))));
+            }
+            d = ad(d, e);
+            d = fm(d, neg(mu(span, k[i])), d);
+            if (rs >> i & 1u) d = zero;
+        }
+        auto& mw = maps[n & 1];
+        mw[warp].m[lane] = m;
+        mw[warp].R[lane] = d;
+        __syncthreads();
+        d = D;
+#pragma unroll
+        for (int w = kWarps - 1; w >= 0; --w) {
+            const F A = mw[w].m[lane].A;
+            if (w == warp) d = D;
+            D = through(A, mw[w].R[lane], D);
+        }
+        for (int w = 0; w < warp; ++w) {
+            const Map<F> o = mw[w].m[lane];
+            h = through(o.A, o.H, h);
+        }
+        F hp[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (rs >> i & 1u) h = zero;
+            hp[i] = h;
+            h = step(h, mu(span, k[i]), unpack<T>(xw[i]));
+        }
+        const int64_t at = (b * a.length + t) * a.dim + c;
+        F dl = zero;
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i) {
+            const F g = mu(span, k[i]), x = unpack<T>(xw[i]), dy = unpack<T>(dw[i]);
+            const F dx0 = sub(x, hp[i]);
+            F e = dy;
+            if (GATE) {
+                const F z = unpack<T>(zw[i]), s = sigmoid_neg(neg(z)), zs = mu(z, s);
+                e = mu(dy, zs);
+                // silu'(z) = s + z s (1 - s)
+                const F ds = fm(zs, sub(one, s), s);
+                if (i < live)
+                    st_word<T>(static_cast<T*>(a.dz) + at + i * a.dim, mu(mu(dy, step(hp[i], g, x)), ds), c, a.dim,
+                               a.words);
+            }
+            d = ad(d, e);                          // dh of step i
+            const F dg = mu(d, dx0);
+            if (i < live) {
+                st_word<T>(static_cast<T*>(a.dx) + at + i * a.dim, mu(g, d), c, a.dim, a.words);
+                st_word<T>(static_cast<T*>(a.dforget) + at + i * a.dim, mu(mu(dg, g), sub(k[i], one)), c, a.dim,
+                           a.words);
+            }
+            dl = fm(dg, k[i], dl);
+            d = fm(d, neg(g), d);
+            if (rs >> i & 1u) d = zero;
+        }
+        dlower = sub(dlower, dl);
+    }
+    if (warp == 0 && a.dinit != nullptr) st_chan(a.dinit + b * a.dim, c, a.dim, D);
+    if (a.part != nullptr) {
+        sums[warp][lane] = dlower;
+        __syncthreads();
+        if (warp == 0) {
+            F s = sums[0][lane];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) s = ad(s, sums[w][lane]);
+            st_chan(a.part + b * a.dim, c, a.dim, s);
+        }
+    }
+}
+
+// dlower[c] = the partial rows added in order.
+__global__ void fold_kernel(const float* part, int64_t rows, int64_t dim, float* out) {
+    const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (c >= dim) return;
+    float s = 0.0f;
+    for (int64_t r = 0; r < rows; ++r) s += part[r * dim + c];
+    out[c] = s;
+}
+
+// ------------------------------------------------------------ one token a row --
+struct StepArgs {
+    int64_t batch, dim, xb, fb, zb, sb, lanes;      // batch strides; lanes per row
+    const void* x; const void* forget; const void* z; const float* lower; float* state; void* y;
+    int words;
+};
+
+template <typename T, bool GATE>
+__global__ void __launch_bounds__(kThreads)
+step_kernel(const StepArgs a) {
+    using F = typename Lane<T>::F;
+    constexpr int E = Lane<T>::E;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= a.batch * a.lanes) return;
+    const int64_t b = i / a.lanes, c = (i % a.lanes) * E;
+    const F x = unpack<T>(ld_word<T>(static_cast<const T*>(a.x) + b * a.xb + c, c, a.dim, a.words));
+    const F f = unpack<T>(ld_word<T>(static_cast<const T*>(a.forget) + b * a.fb + c, c, a.dim, a.words));
+    F z = same<F>(0.0f), span, h;
+    if (GATE) z = unpack<T>(ld_word<T>(static_cast<const T*>(a.z) + b * a.zb + c, c, a.dim, a.words));
+    ld_chan(a.lower, c, a.dim, 0.0f, span);
+    ld_chan(a.state + b * a.sb, c, a.dim, 0.0f, h);
+    const F g = mu(sub(same<F>(1.0f), span), sigmoid_neg(f));
+    h = step(h, g, x);
+    st_chan(a.state + b * a.sb, c, a.dim, h);
+    if (GATE) h = mu(h, mu(z, sigmoid_neg(neg(z))));
+    st_word<T>(static_cast<T*>(a.y) + b * a.dim + c, h, c, a.dim, a.words);
+}
+
+// ------------------------------------------------------------------- host ----
+static int64_t esize(int dtype) { return dtype == SSM_F32 ? 4 : 2; }
+static bool al(const void* p, int64_t b) { return (reinterpret_cast<uintptr_t>(p) % b) == 0; }
+
+static int validate(const ssm_gated_recurrence_params* p) {
+    if (p == nullptr) return fail(SSM_ERR_INVALID, "gated_linear_recurrence: null params");
+    if (p->batch < 0 || p->length < 0 || p->dim < 1)
+        return fail(SSM_ERR_INVALID, "gated_linear_recurrence: batch, length and dim");
+    if (p->batch > 65535 || p->length > INT32_MAX || p->dim > INT32_MAX)
+        return fail(SSM_ERR_UNSUPPORTED, "gated_linear_recurrence: batch above 65535, or length or dim above 2^31 - 1");
+    if (p->dtype < SSM_F32 || p->dtype > SSM_F16) return fail(SSM_ERR_UNSUPPORTED, "gated_linear_recurrence: dtype");
+    for (int64_t s : {p->x_token_stride, p->forget_token_stride, p->z_token_stride, p->dy_token_stride})
+        if (s && s < p->dim) return fail(SSM_ERR_INVALID, "gated_linear_recurrence: a token stride is below dim");
+    return SSM_OK;
+}
+
+static Args args_of(const ssm_gated_recurrence_params* p) {
+    Args a{};
+    a.batch = p->batch; a.length = p->length; a.dim = p->dim;
+    a.chunks = ceil_div(p->length, kChunk);
+    auto token = [&](int64_t s) { return s ? s : p->dim; };
+    auto row = [&](int64_t s, int64_t t) { return s ? s : t * p->length; };
+    a.xt = token(p->x_token_stride); a.xb = row(p->x_batch_stride, a.xt);
+    a.ft = token(p->forget_token_stride); a.fb = row(p->forget_batch_stride, a.ft);
+    a.zt = token(p->z_token_stride); a.zb = row(p->z_batch_stride, a.zt);
+    a.dyt = token(p->dy_token_stride); a.dyb = row(p->dy_batch_stride, a.dyt);
+    a.x = p->x; a.forget = p->forget; a.z = p->z;
+    a.lower = p->lower; a.init = p->initial_state; a.reset = p->reset;
+    a.y = p->y; a.final_state = p->final_state; a.states = p->states;
+    a.dy = p->dy; a.dfinal = p->dfinal;
+    a.dx = p->dx; a.dforget = p->dforget; a.dz = p->dz; a.dinit = p->dinitial;
+    a.words = 1;
+    if (p->dtype != SSM_F32) {
+        for (const void* q : {p->x, p->forget, p->z, (const void*)p->y, p->dy, (const void*)p->dx,
+                              (const void*)p->dforget, (const void*)p->dz})
+            if (!al(q, 4)) a.words = 0;
+        for (int64_t s : {a.dim, a.xt, a.xb, a.ft, a.fb, p->z ? a.zt : 0, p->z ? a.zb : 0, p->dy ? a.dyt : 0,
+                          p->dy ? a.dyb : 0})
+            if (s & 1) a.words = 0;
+    }
+    return a;
+}
+
+template <typename T>
+static void launch(const Args& a, bool bwd, cudaStream_t st) {
+    const dim3 grid((unsigned)ceil_div(a.dim, 32 * Lane<T>::E), (unsigned)a.batch);
+    if (bwd) {
+        if (a.z) bwd_kernel<T, true><<<grid, kThreads, 0, st>>>(a);
+        else bwd_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
+    } else {
+        if (a.z) fwd_kernel<T, true><<<grid, kThreads, 0, st>>>(a);
+        else fwd_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
+    }
+}
+
+static void launch_any(int dtype, const Args& a, bool bwd, cudaStream_t st) {
+    if (dtype == SSM_F32) launch<float>(a, bwd, st);
+    else if (dtype == SSM_BF16) launch<__nv_bfloat16>(a, bwd, st);
+    else launch<__half>(a, bwd, st);
+}
+
+template <typename T>
+static void launch_step(const StepArgs& a, cudaStream_t st) {
+    const unsigned grid = (unsigned)ceil_div(a.batch * a.lanes, kThreads);
+    if (a.z) step_kernel<T, true><<<grid, kThreads, 0, st>>>(a);
+    else step_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
+}
+
+}  // namespace glr
+}  // namespace ssm
+
+using namespace ssm;
+using namespace ssm::glr;
+
+extern "C" int ssm_gated_recurrence_sizes(const ssm_gated_recurrence_params* p, size_t* states_bytes,
+                                          size_t* workspace_bytes) {
+    if (int s = validate(p)) return s;
+    if (states_bytes) *states_bytes = (size_t)(p->batch * ceil_div(p->length, kChunk) * p->dim) * 4;
+    if (workspace_bytes) *workspace_bytes = (size_t)(p->batch * p->dim) * 4;
+    return SSM_OK;
+}
+
+extern "C" int ssm_gated_recurrence_fwd(const ssm_gated_recurrence_params* p, void* stream) {
+    if (int s = validate(p)) return s;
+    if (p->batch == 0) return SSM_OK;
+    if (!p->final_state || (p->length && (!p->x || !p->forget || !p->y)))
+        return fail(SSM_ERR_INVALID, "gated_linear_recurrence fwd: null pointer");
+    launch_any(p->dtype, args_of(p), false, static_cast<cudaStream_t>(stream));
+    return check_launch("gated_linear_recurrence fwd");
+}
+
+extern "C" int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, void* stream) {
+    if (int s = validate(p)) return s;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p->batch == 0) {
+        if (p->dlower && cudaMemsetAsync(p->dlower, 0, (size_t)p->dim * 4, st))
+            return check_launch("gated_linear_recurrence bwd: zero dlower");
+        return SSM_OK;
+    }
+    if (p->length && (!p->x || !p->forget || !p->dy || !p->states || !p->dx || !p->dforget || (p->z && !p->dz)))
+        return fail(SSM_ERR_INVALID, "gated_linear_recurrence bwd: null pointer");
+    Args a = args_of(p);
+    if (p->dlower) {
+        size_t need = 0;
+        ssm_gated_recurrence_sizes(p, nullptr, &need);
+        if (!p->workspace || p->workspace_bytes < need)
+            return fail(SSM_ERR_WORKSPACE, "gated_linear_recurrence bwd: workspace smaller than ssm_gated_recurrence_sizes");
+        a.part = static_cast<float*>(p->workspace);
+    }
+    launch_any(p->dtype, a, true, st);
+    if (int s = check_launch("gated_linear_recurrence bwd")) return s;
+    if (p->dlower) {
+        fold_kernel<<<(unsigned)ceil_div(a.dim, 256), 256, 0, st>>>(a.part, a.batch, a.dim, p->dlower);
+        return check_launch("gated_linear_recurrence bwd: fold");
+    }
+    return SSM_OK;
+}
+
+extern "C" int ssm_gated_recurrence_step(const ssm_gated_recurrence_step_params* p, void* stream) {
+    if (p == nullptr) return fail(SSM_ERR_INVALID, "gated_linear_recurrence_update: null params");
+    if (p->batch < 0 || p->dim < 1) return fail(SSM_ERR_INVALID, "gated_linear_recurrence_update: batch and dim");
+    if (p->dtype < SSM_F32 || p->dtype > SSM_F16)
+        return fail(SSM_ERR_UNSUPPORTED, "gated_linear_recurrence_update: dtype");
+    if (p->batch > INT32_MAX || p->dim > INT32_MAX || p->batch * p->dim > ((int64_t)1 << 38))
+        return fail(SSM_ERR_UNSUPPORTED, "gated_linear_recurrence_update: too large");
+    if (p->batch == 0) return SSM_OK;
+    if (!p->x || !p->forget || !p->state || !p->y)
+        return fail(SSM_ERR_INVALID, "gated_linear_recurrence_update: null pointer");
+    StepArgs a{};
+    a.batch = p->batch; a.dim = p->dim;
+    auto row = [&](int64_t s) { return s ? s : p->dim; };
+    a.xb = row(p->x_batch_stride); a.fb = row(p->forget_batch_stride); a.zb = row(p->z_batch_stride);
+    a.sb = row(p->state_batch_stride);
+    for (int64_t s : {a.xb, a.fb, a.zb, a.sb})
+        if (s < p->dim) return fail(SSM_ERR_INVALID, "gated_linear_recurrence_update: a batch stride is below dim");
+    a.x = p->x; a.forget = p->forget; a.z = p->z; a.lower = p->lower; a.state = p->state; a.y = p->y;
+    a.lanes = ceil_div(p->dim * esize(p->dtype), 4);
+    a.words = 1;
+    if (p->dtype != SSM_F32) {
+        for (const void* q : {p->x, p->forget, p->z, (const void*)p->y}) if (!al(q, 4)) a.words = 0;
+        for (int64_t s : {a.dim, a.xb, a.fb, p->z ? a.zb : 0}) if (s & 1) a.words = 0;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p->dtype == SSM_F32) launch_step<float>(a, st);
+    else if (p->dtype == SSM_BF16) launch_step<__nv_bfloat16>(a, st);
+    else launch_step<__half>(a, st);
+    return check_launch("gated_linear_recurrence_update");
+}

@@ -34,3 +34,22 @@ def add_rmsnorm_grads_ref(dy, dstream, stream, weight, eps=1e-5):
     if dstream is not None:
         d = d + dstream.double()
     return d, (up * xh).reshape(-1, w.numel()).sum(0)
+
+
+def gated_recurrence_ref(x, forget, z=None, lower=None, init=None, reset=None):
+    """(y, final): the recurrence step by step; differentiable in float64."""
+    batch, length, dim = x.shape
+    low = torch.zeros(dim, dtype=torch.float64) if lower is None else lower
+    gate = low + (1 - low) * torch.sigmoid(forget)
+    write = (1 - low) * torch.sigmoid(-forget)
+    h = torch.zeros(batch, dim, dtype=torch.float64) if init is None else init
+    hs = []
+    for t in range(length):
+        if reset is not None:
+            h = torch.where(reset[:, t, None].bool(), torch.zeros_like(h), h)
+        h = gate[:, t] * h + write[:, t] * x[:, t]
+        hs.append(h)
+    y = torch.stack(hs, 1) if hs else x.new_zeros(batch, 0, dim)
+    if z is not None:
+        y = y * (z * torch.sigmoid(z))
+    return y, h
