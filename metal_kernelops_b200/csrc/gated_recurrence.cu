@@ -21,22 +21,34 @@
 // channels (a lane: one 4-byte word, two 16-bit channels or one fp32 channel),
 // holds them in registers, and reduces them to (A, H); the warps' maps meet in
 // shared memory, each warp composes those before it and walks its steps a second
-// time from the right start.  A CTA's kWarps warps make a chunk, and the CTA goes
-// through the chunks of its rows in order.
+// time from the right start.  A CTA's kWarps warps make a chunk.  Where the channel
+// tiles of all batch rows do not fill the GPU, a cluster of CTAs takes consecutive
+// chunks of one tile at a time, and its CTAs exchange their chunks' maps through
+// distributed shared memory, one cluster barrier for each such round; the inputs
+// are still read once.  Chunks come through a ring of shared-memory stages that TMA
+// fills ahead (rows that do not start on 16-byte boundaries are read directly).
 // A composition whose A is exactly 0 (a reset) takes H alone: a state that is not
 // finite does not pass a reset.
 // The forward saves the state that enters each chunk, in fp32, for the backward,
 // which recomputes the chunk's states from it.
+#include <cooperative_groups.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <climits>
+#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace ssm {
 namespace glr {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kSteps = 8, kChunk = kWarps * kSteps;
+constexpr int kTile = kChunk * 128;                 // bytes of one tensor's chunk: 128-byte rows
+constexpr int kMaxCluster = 8;
 
 struct Args {
     int64_t batch, length, dim, chunks;
@@ -47,7 +59,23 @@ struct Args {
     const void* dy; const float* dfinal;
     void* dx; void* dforget; void* dz; float* dinit; float* part;
     int words;                                      // 4-byte accesses are aligned
+    int* status;
 };
+
+// x, forget, z, dy as (channel, token, batch row)
+struct TmaArgs {
+    Args a;
+    alignas(64) CUtensorMap m[4];
+};
+
+__device__ int g_glr_error;
+
+// A bounded wait ran out: record the code in the device's flag and in the
+// call's status word; the first failure wins.
+__device__ __forceinline__ void report(const Args& a, int code) {
+    atomicCAS(&g_glr_error, 0, code);
+    if (a.status) atomicCAS(a.status, 0, code);
+}
 
 // ------------------------------------------------- one or two channels a lane --
 template <typename T> struct Lane { using F = float2; static constexpr int E = 2; };
@@ -153,33 +181,99 @@ __device__ __forceinline__ void ld_steps(const void* base, int64_t row, int64_t 
     for (int i = 0; i < kSteps; ++i) w[i] = i < n ? ld_word<T>(p + i * stride, c, a.dim, a.words) : 0u;
 }
 
-template <typename F> struct Map { F A, H; };
+// The ring of chunk tiles in shared memory that TMA fills: stage s holds NT
+// tensors' chunks, a warp's steps being kSteps consecutive 128-byte rows of each.
+// Thread 0 issues; the wait of a stage is every thread's.
+template <int NT, int ST>
+struct Ring {
+    uint8_t* base;                  // ST * NT * kTile bytes, then ST mbarriers
+    static constexpr size_t bytes = (size_t)ST * NT * kTile + ST * 8;
+    __device__ __forceinline__ uint32_t bar(int s) const {
+        return tc::smem_u32(base + (size_t)ST * NT * kTile) + s * 8;
+    }
+    __device__ __forceinline__ void init() const {
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < ST; ++s) tc::mbar_init(bar(s), 1);
+            tc::fence_mbar_init();
+        }
+        __syncthreads();
+    }
+    // The chunk at token t of batch row b into stage s: tensor i of the stage is map which[i].
+    __device__ __forceinline__ void load(const TmaArgs& ta, int s, int c0, int64_t t, int b, const int* which) const {
+        tc::mbar_expect_tx(bar(s), NT * kTile);
+        for (int i = 0; i < NT; ++i)
+            tc::tma_load3(tc::smem_u32(base + (s * NT + i) * kTile), &ta.m[which[i]], c0, (int)t, b, bar(s));
+    }
+    __device__ __forceinline__ void read(int s, int i, uint32_t* w) const {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (s * NT + i) * kTile) + threadIdx.x / 32 * kSteps * 32 +
+                            (threadIdx.x & 31);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) w[k] = p[k * 32];
+    }
+};
 
-template <typename T, bool GATE>
-__global__ void __launch_bounds__(kThreads)
-fwd_kernel(const Args a) {
+template <typename F> struct Map { F A, H; };
+template <typename F> __device__ __forceinline__ Map<F> then(const Map<F>& first, const Map<F>& next) {
+    return {mu(first.A, next.A), through(next.A, next.H, first.H)};
+}
+
+// A cluster of C CTAs takes C consecutive chunks at a time: its CTAs exchange
+// their chunks' maps through each other's shared memory, once a round.
+__device__ __forceinline__ int cluster_size() { return (int)cooperative_groups::this_cluster().num_blocks(); }
+
+template <typename T, bool GATE, bool TMA, int ST>
+__global__ void __launch_bounds__(kThreads, 3)
+fwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
-    constexpr int E = Lane<T>::E;
+    constexpr int E = Lane<T>::E, NT = GATE ? 3 : 2;
+    const Args& a = ta.a;
     __shared__ Map<F> maps[2][kWarps][32];
+    __shared__ Map<F> far[2][kMaxCluster][32];
+    extern __shared__ __align__(128) uint8_t smem[];
+    const Ring<NT, ST> ring{smem};
+    const int which[3] = {0, 1, 2};
+    const auto cluster = cooperative_groups::this_cluster();
+    const int C = cluster_size(), rank = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t b = blockIdx.y, c = ((int64_t)blockIdx.x * 32 + lane) * E;
+    const int64_t b = blockIdx.y, tile = blockIdx.x / C, c = (tile * 32 + lane) * E;
+    const int64_t rounds = (a.chunks + C - 1) / C;
+    if (C > 1) cluster.sync();                          // every CTA's shared memory is there to write to
+    if constexpr (TMA) {
+        ring.init();
+        if (threadIdx.x == 0)
+            for (int s = 0; s < ST && s < rounds; ++s)
+                ring.load(ta, s, (int)(tile * 32 * E), ((int64_t)s * C + rank) * kChunk, (int)b, which);
+    }
     F span, S;
     ld_chan(a.lower, c, a.dim, 0.0f, span);
     span = sub(same<F>(1.0f), span);
     ld_chan(a.init ? a.init + b * a.dim : nullptr, c, a.dim, 0.0f, S);
-    for (int64_t n = 0; n < a.chunks; ++n) {
-        const int64_t t = n * kChunk + warp * kSteps;
+    for (int64_t n = 0; n < rounds; ++n) {
+        const int64_t chunk = n * C + rank, t = chunk * kChunk + warp * kSteps;
         const int live = (int)max64(0, min64(kSteps, a.length - t));
-        uint32_t xw[kSteps], fw[kSteps], zw[kSteps];
-        ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
-        ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
-        if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
-        const uint32_t rs = reset_mask(a.reset, b * a.length, t, a.length);
+        uint32_t xw[kSteps], zw[kSteps];
         F g[kSteps];
+        const uint32_t rs = reset_mask(a.reset, b * a.length, t, a.length);
+        {
+            uint32_t fw[kSteps];
+            if constexpr (TMA) {
+                const int s = (int)(n % ST);
+                if (!tc::mbar_wait(ring.bar(s), (uint32_t)(n / ST) & 1u) && lane == 0) report(a, 111);
+                ring.read(s, 0, xw);
+                ring.read(s, 1, fw);
+                if (GATE) ring.read(s, 2, zw);
+            } else {
+                ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
+                ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
+                if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                g[i] = i < live ? mu(span, sigmoid_neg(unpack<T>(fw[i]))) : same<F>(0.0f);
+        }
         Map<F> m{same<F>(1.0f), same<F>(0.0f)};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            g[i] = i < live ? mu(span, sigmoid_neg(unpack<T>(fw[i]))) : same<F>(0.0f);
             if (rs >> i & 1u) m = {same<F>(0.0f), same<F>(0.0f)};
             m.H = step(m.H, g[i], unpack<T>(xw[i]));
             m.A = fm(m.A, neg(g[i]), m.A);
@@ -187,14 +281,35 @@ fwd_kernel(const Args a) {
         Map<F>(*mw)[32] = maps[n & 1];
         mw[warp][lane] = m;
         __syncthreads();
-        if (a.states != nullptr && warp == 0)
-            st_chan(a.states + (b * a.chunks + n) * a.dim, c, a.dim, S);
-        F h = S;
+        // every warp has its words in registers: the stage is free
+        if (TMA && threadIdx.x == 0 && n + ST < rounds)
+            ring.load(ta, (int)(n % ST), (int)(tile * 32 * E), ((n + ST) * C + rank) * kChunk, (int)b, which);
+        F h;
+        if (C == 1) {
+            if (a.states != nullptr && warp == 0) st_chan(a.states + (b * a.chunks + chunk) * a.dim, c, a.dim, S);
+            h = S;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const Map<F> o = mw[w][lane];
-            if (w == warp) h = S;
-            S = through(o.A, o.H, S);
+            for (int w = 0; w < kWarps; ++w) {
+                const Map<F> o = mw[w][lane];
+                if (w == warp) h = S;
+                S = through(o.A, o.H, S);
+            }
+        } else {
+            Map<F> before{same<F>(1.0f), same<F>(0.0f)};
+            for (int w = 0; w < warp; ++w) before = then(before, mw[w][lane]);
+            if (warp == kWarps - 1) {
+                const Map<F> all = then(before, m);
+                for (int r = 0; r < C; ++r) cluster.map_shared_rank(&far[n & 1][0][0], r)[rank * 32 + lane] = all;
+            }
+            cluster.sync();
+            for (int r = 0; r < C; ++r) {
+                if (r == rank) h = S;
+                const Map<F> o = far[n & 1][r][lane];
+                S = through(o.A, o.H, S);
+            }
+            if (a.states != nullptr && warp == 0 && chunk < a.chunks)
+                st_chan(a.states + (b * a.chunks + chunk) * a.dim, c, a.dim, h);
+            h = through(before.A, before.H, h);
         }
         T* y = static_cast<T*>(a.y) + (b * a.length + t) * a.dim + c;
 #pragma unroll
@@ -209,40 +324,67 @@ fwd_kernel(const Args a) {
             if (i < live) st_word<T>(y + i * a.dim, o, c, a.dim, a.words);
         }
     }
-    if (warp == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
+    if (warp == 0 && rank == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
 }
 
-template <typename T, bool GATE>
-__global__ void __launch_bounds__(kThreads)
-bwd_kernel(const Args a) {
+template <typename T, bool GATE, bool TMA, int ST>
+__global__ void __launch_bounds__(kThreads, 2)
+bwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
-    constexpr int E = Lane<T>::E;
+    constexpr int E = Lane<T>::E, NT = GATE ? 4 : 3;
+    const Args& a = ta.a;
     __shared__ struct { Map<F> m[32]; F R[32]; } maps[2][kWarps];
+    __shared__ Map<F> far[2][kMaxCluster][32];          // H holds R here
     __shared__ F sums[kWarps][32];
+    extern __shared__ __align__(128) uint8_t smem[];
+    const Ring<NT, ST> ring{smem};
+    const int which[4] = {0, 1, 3, 2};                  // x, forget, dy, z
+    const auto cluster = cooperative_groups::this_cluster();
+    const int C = cluster_size(), rank = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t b = blockIdx.y, c = ((int64_t)blockIdx.x * 32 + lane) * E;
+    const int64_t b = blockIdx.y, tile = blockIdx.x / C, c = (tile * 32 + lane) * E;
+    const int64_t rounds = (a.chunks + C - 1) / C;
+    if (C > 1) cluster.sync();                          // every CTA's shared memory is there to write to
+    if constexpr (TMA) {
+        ring.init();
+        if (threadIdx.x == 0)
+            for (int s = 0; s < ST && s < rounds; ++s)
+                ring.load(ta, s, (int)(tile * 32 * E), ((rounds - 1 - s) * C + rank) * kChunk, (int)b, which);
+    }
     const F one = same<F>(1.0f), zero = same<F>(0.0f);
     F span, D;
     ld_chan(a.lower, c, a.dim, 0.0f, span);
     span = sub(one, span);
     ld_chan(a.dfinal ? a.dfinal + b * a.dim : nullptr, c, a.dim, 0.0f, D);
     F dlower = zero;
-    for (int64_t n = a.chunks - 1; n >= 0; --n) {
-        const int64_t t = n * kChunk + warp * kSteps;
+    for (int64_t turn = 0; turn < rounds; ++turn) {
+        const int64_t chunk = (rounds - 1 - turn) * C + rank, t = chunk * kChunk + warp * kSteps;
         const int live = (int)max64(0, min64(kSteps, a.length - t));
-        uint32_t xw[kSteps], fw[kSteps], zw[kSteps], dw[kSteps];
-        ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
-        ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
-        if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
-        ld_steps<T>(a.dy, b * a.dyb, a.dyt, t, live, c, a, dw);
-        F h;
-        ld_chan(a.states + (b * a.chunks + n) * a.dim, c, a.dim, 0.0f, h);
+        uint32_t xw[kSteps], zw[kSteps], dw[kSteps];
+        F k[kSteps], h;
         const uint32_t rs = reset_mask(a.reset, b * a.length, t, a.length);
-        F k[kSteps];
+        ld_chan(chunk < a.chunks ? a.states + (b * a.chunks + chunk) * a.dim : nullptr, c, a.dim, 0.0f, h);
+        {
+            uint32_t fw[kSteps];
+            if constexpr (TMA) {
+                const int s = (int)(turn % ST);
+                if (!tc::mbar_wait(ring.bar(s), (uint32_t)(turn / ST) & 1u) && lane == 0) report(a, 112);
+                ring.read(s, 0, xw);
+                ring.read(s, 1, fw);
+                ring.read(s, 2, dw);
+                if (GATE) ring.read(s, 3, zw);
+            } else {
+                ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
+                ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
+                if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
+                ld_steps<T>(a.dy, b * a.dyb, a.dyt, t, live, c, a, dw);
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) k[i] = i < live ? sigmoid_neg(unpack<T>(fw[i])) : zero;
+        }
         Map<F> m{one, zero};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            k[i] = i < live ? sigmoid_neg(unpack<T>(fw[i])) : zero;
             const F g = mu(span, k[i]);
             if (rs >> i & 1u) m = {zero, zero};
             m.H = step(m.H, g, unpack<T>(xw[i]));
@@ -260,16 +402,35 @@ bwd_kernel(const Args a) {
             d = fm(d, neg(mu(span, k[i])), d);
             if (rs >> i & 1u) d = zero;
         }
-        auto& mw = maps[n & 1];
+        auto& mw = maps[turn & 1];
         mw[warp].m[lane] = m;
         mw[warp].R[lane] = d;
         __syncthreads();
-        d = D;
+        if (TMA && threadIdx.x == 0 && turn + ST < rounds)
+            ring.load(ta, (int)(turn % ST), (int)(tile * 32 * E), ((rounds - 1 - turn - ST) * C + rank) * kChunk, (int)b,
+                      which);
+        if (C == 1) {
+            d = D;
 #pragma unroll
-        for (int w = kWarps - 1; w >= 0; --w) {
-            const F A = mw[w].m[lane].A;
-            if (w == warp) d = D;
-            D = through(A, mw[w].R[lane], D);
+            for (int w = kWarps - 1; w >= 0; --w) {
+                const F A = mw[w].m[lane].A;
+                if (w == warp) d = D;
+                D = through(A, mw[w].R[lane], D);
+            }
+        } else {
+            Map<F> after{one, zero};
+            for (int w = kWarps - 1; w > warp; --w) after = then(after, Map<F>{mw[w].m[lane].A, mw[w].R[lane]});
+            if (warp == 0) {
+                const Map<F> all = then(after, Map<F>{m.A, d});
+                for (int r = 0; r < C; ++r) cluster.map_shared_rank(&far[turn & 1][0][0], r)[rank * 32 + lane] = all;
+            }
+            cluster.sync();
+            for (int r = C - 1; r >= 0; --r) {
+                if (r == rank) d = D;
+                const Map<F> o = far[turn & 1][r][lane];
+                D = through(o.A, o.H, D);
+            }
+            d = through(after.A, after.H, d);
         }
         for (int w = 0; w < warp; ++w) {
             const Map<F> o = mw[w].m[lane];
@@ -287,7 +448,6 @@ bwd_kernel(const Args a) {
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
             const F g = mu(span, k[i]), x = unpack<T>(xw[i]), dy = unpack<T>(dw[i]);
-            const F dx0 = sub(x, hp[i]);
             F e = dy;
             if (GATE) {
                 const F z = unpack<T>(zw[i]), s = sigmoid_neg(neg(z)), zs = mu(z, s);
@@ -299,7 +459,7 @@ bwd_kernel(const Args a) {
                                a.words);
             }
             d = ad(d, e);                          // dh of step i
-            const F dg = mu(d, dx0);
+            const F dg = mu(d, sub(x, hp[i]));
             if (i < live) {
                 st_word<T>(static_cast<T*>(a.dx) + at + i * a.dim, mu(g, d), c, a.dim, a.words);
                 st_word<T>(static_cast<T*>(a.dforget) + at + i * a.dim, mu(mu(dg, g), sub(k[i], one)), c, a.dim,
@@ -311,7 +471,7 @@ bwd_kernel(const Args a) {
         }
         dlower = sub(dlower, dl);
     }
-    if (warp == 0 && a.dinit != nullptr) st_chan(a.dinit + b * a.dim, c, a.dim, D);
+    if (warp == 0 && rank == 0 && a.dinit != nullptr) st_chan(a.dinit + b * a.dim, c, a.dim, D);
     if (a.part != nullptr) {
         sums[warp][lane] = dlower;
         __syncthreads();
@@ -319,7 +479,7 @@ bwd_kernel(const Args a) {
             F s = sums[0][lane];
 #pragma unroll
             for (int w = 1; w < kWarps; ++w) s = ad(s, sums[w][lane]);
-            st_chan(a.part + b * a.dim, c, a.dim, s);
+            st_chan(a.part + (b * C + rank) * a.dim, c, a.dim, s);
         }
     }
 }
@@ -392,6 +552,7 @@ static Args args_of(const ssm_gated_recurrence_params* p) {
     a.y = p->y; a.final_state = p->final_state; a.states = p->states;
     a.dy = p->dy; a.dfinal = p->dfinal;
     a.dx = p->dx; a.dforget = p->dforget; a.dz = p->dz; a.dinit = p->dinitial;
+    a.status = p->status;
     a.words = 1;
     if (p->dtype != SSM_F32) {
         for (const void* q : {p->x, p->forget, p->z, (const void*)p->y, p->dy, (const void*)p->dx,
@@ -404,22 +565,118 @@ static Args args_of(const ssm_gated_recurrence_params* p) {
     return a;
 }
 
-template <typename T>
-static void launch(const Args& a, bool bwd, cudaStream_t st) {
-    const dim3 grid((unsigned)ceil_div(a.dim, 32 * Lane<T>::E), (unsigned)a.batch);
-    if (bwd) {
-        if (a.z) bwd_kernel<T, true><<<grid, kThreads, 0, st>>>(a);
-        else bwd_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
-    } else {
-        if (a.z) fwd_kernel<T, true><<<grid, kThreads, 0, st>>>(a);
-        else fwd_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
-    }
+static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+        else
+            cudaGetLastError();
+    });
+    return fn;
 }
 
-static void launch_any(int dtype, const Args& a, bool bwd, cudaStream_t st) {
-    if (dtype == SSM_F32) launch<float>(a, bwd, st);
-    else if (dtype == SSM_BF16) launch<__nv_bfloat16>(a, bwd, st);
-    else launch<__half>(a, bwd, st);
+// (batch, length, dim) as (channel, token, batch row); box: one chunk of 128-byte rows.
+static int encode(CUtensorMap* m, const void* base, int64_t token, int64_t row, int dtype, const Args& a) {
+    const int64_t es = esize(dtype);
+    cuuint64_t dims[3] = {(cuuint64_t)a.dim, (cuuint64_t)a.length, (cuuint64_t)a.batch};
+    // a single row's stride is never used, but has to be a valid one
+    cuuint64_t strides[2] = {(cuuint64_t)(token * es), (cuuint64_t)((a.batch > 1 ? row : token) * es)};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)kChunk, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUtensorMapDataType type = dtype == SSM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : dtype == SSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = encoder()(m, type, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return SSM_OK;
+    return fail(SSM_ERR_CUDA, "gated_linear_recurrence: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+}
+
+// TMA reads rows that start on 16-byte boundaries.
+static bool tma_ok(const Args& a, int dtype, bool bwd) {
+    const int64_t es = esize(dtype);
+    auto ok = [&](const void* p, int64_t token, int64_t row) {
+        return p == nullptr || (al(p, 16) && (token * es) % 16 == 0 &&
+                                (a.batch == 1 || (row * es) % 16 == 0) && token * es < ((int64_t)1 << 40) &&
+                                (a.batch == 1 || row * es < ((int64_t)1 << 40)));
+    };
+    return encoder() && a.length > 0 && ok(a.x, a.xt, a.xb) && ok(a.forget, a.ft, a.fb) && ok(a.z, a.zt, a.zb) &&
+           (!bwd || ok(a.dy, a.dyt, a.dyb));
+}
+
+// CTAs of a cluster: as many (a power of two, up to 8, no more than chunks) as
+// bring the grid to two CTAs per SM.
+static int cluster_of(const ssm_gated_recurrence_params* p) {
+    const int64_t tiles = ceil_div(p->dim * esize(p->dtype), 128), chunks = ceil_div(p->length, kChunk);
+    int c = 1;
+    while (c < kMaxCluster && 2 * c <= chunks && tiles * p->batch * c < 148 * 2) c *= 2;
+    return c;
+}
+
+template <typename K>
+static int launch_kernel(K kernel, const TmaArgs& ta, unsigned tiles, int cluster, size_t smem, cudaStream_t st,
+                         const char* what) {
+    if (smem && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return check_launch(what);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles * cluster, (unsigned)ta.a.batch);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, ta);
+    return check_launch(what);
+}
+
+constexpr int kFwdStages = 2, kBwdStages = 2;
+
+template <typename T, bool GATE>
+static int launch(const TmaArgs& ta, bool bwd, bool tma, int cluster, cudaStream_t st) {
+    const unsigned tiles = (unsigned)ceil_div(ta.a.dim, 32 * Lane<T>::E);
+    constexpr size_t fs = Ring<GATE ? 3 : 2, kFwdStages>::bytes, bs = Ring<GATE ? 4 : 3, kBwdStages>::bytes;
+    if (bwd) {
+        const char* what = "gated_linear_recurrence bwd";
+        if (tma) return launch_kernel(bwd_kernel<T, GATE, true, kBwdStages>, ta, tiles, cluster, bs, st, what);
+        return launch_kernel(bwd_kernel<T, GATE, false, kBwdStages>, ta, tiles, cluster, 0, st, what);
+    }
+    const char* what = "gated_linear_recurrence fwd";
+    if (tma) return launch_kernel(fwd_kernel<T, GATE, true, kFwdStages>, ta, tiles, cluster, fs, st, what);
+    return launch_kernel(fwd_kernel<T, GATE, false, kFwdStages>, ta, tiles, cluster, 0, st, what);
+}
+
+template <typename T>
+static int launch_gate(const TmaArgs& ta, bool bwd, bool tma, int cluster, cudaStream_t st) {
+    return ta.a.z ? launch<T, true>(ta, bwd, tma, cluster, st) : launch<T, false>(ta, bwd, tma, cluster, st);
+}
+
+static int launch_any(const ssm_gated_recurrence_params* p, const Args& a, bool bwd, cudaStream_t st) {
+    TmaArgs ta{};
+    ta.a = a;
+    const bool tma = tma_ok(a, p->dtype, bwd);
+    if (tma) {
+        if (int s = ensure_context("gated_linear_recurrence")) return s;
+        if (int s = encode(&ta.m[0], a.x, a.xt, a.xb, p->dtype, a)) return s;
+        if (int s = encode(&ta.m[1], a.forget, a.ft, a.fb, p->dtype, a)) return s;
+        if (a.z)
+            if (int s = encode(&ta.m[2], a.z, a.zt, a.zb, p->dtype, a)) return s;
+        if (bwd)
+            if (int s = encode(&ta.m[3], a.dy, a.dyt, a.dyb, p->dtype, a)) return s;
+    }
+    const int cluster = cluster_of(p);
+    if (p->dtype == SSM_F32) return launch_gate<float>(ta, bwd, tma, cluster, st);
+    if (p->dtype == SSM_BF16) return launch_gate<__nv_bfloat16>(ta, bwd, tma, cluster, st);
+    return launch_gate<__half>(ta, bwd, tma, cluster, st);
 }
 
 template <typename T>
@@ -435,11 +692,23 @@ static void launch_step(const StepArgs& a, cudaStream_t st) {
 using namespace ssm;
 using namespace ssm::glr;
 
+// The kernels' error flag on the current device, read and cleared; called by
+// ssm_take_kernel_error.
+int ssm_glr_take_error() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, ssm::glr::g_glr_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(ssm::glr::g_glr_error, &zero, sizeof(int));
+    }
+    return v;
+}
+
 extern "C" int ssm_gated_recurrence_sizes(const ssm_gated_recurrence_params* p, size_t* states_bytes,
                                           size_t* workspace_bytes) {
     if (int s = validate(p)) return s;
     if (states_bytes) *states_bytes = (size_t)(p->batch * ceil_div(p->length, kChunk) * p->dim) * 4;
-    if (workspace_bytes) *workspace_bytes = (size_t)(p->batch * p->dim) * 4;
+    if (workspace_bytes) *workspace_bytes = (size_t)(p->batch * cluster_of(p) * p->dim) * 4;
     return SSM_OK;
 }
 
@@ -448,8 +717,7 @@ extern "C" int ssm_gated_recurrence_fwd(const ssm_gated_recurrence_params* p, vo
     if (p->batch == 0) return SSM_OK;
     if (!p->final_state || (p->length && (!p->x || !p->forget || !p->y)))
         return fail(SSM_ERR_INVALID, "gated_linear_recurrence fwd: null pointer");
-    launch_any(p->dtype, args_of(p), false, static_cast<cudaStream_t>(stream));
-    return check_launch("gated_linear_recurrence fwd");
+    return launch_any(p, args_of(p), false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, void* stream) {
@@ -470,10 +738,9 @@ extern "C" int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, vo
             return fail(SSM_ERR_WORKSPACE, "gated_linear_recurrence bwd: workspace smaller than ssm_gated_recurrence_sizes");
         a.part = static_cast<float*>(p->workspace);
     }
-    launch_any(p->dtype, a, true, st);
-    if (int s = check_launch("gated_linear_recurrence bwd")) return s;
+    if (int s = launch_any(p, a, true, st)) return s;
     if (p->dlower) {
-        fold_kernel<<<(unsigned)ceil_div(a.dim, 256), 256, 0, st>>>(a.part, a.batch, a.dim, p->dlower);
+        fold_kernel<<<(unsigned)ceil_div(a.dim, 256), 256, 0, st>>>(a.part, a.batch * cluster_of(p), a.dim, p->dlower);
         return check_launch("gated_linear_recurrence bwd: fold");
     }
     return SSM_OK;

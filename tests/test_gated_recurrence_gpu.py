@@ -87,6 +87,10 @@ CASES = [  # batch, length, dim, dtype, gate, lower, initial state, reset
     (5, 130, 2, BF16, False, False, True, True),
     (1, 8200, 256, BF16, True, True, True, True),
     (1, 3000, 1024, F16, True, True, True, False),
+    (5, 200, 4096, BF16, True, True, True, True),          # tiles enough without clusters
+    (6, 200, 2000, F32, True, True, True, False),
+    (1, 1000, 4608, BF16, True, False, True, True),        # clusters of four and of two
+    (1, 500, 9472, BF16, False, True, False, True),
 ]
 
 
