@@ -6,11 +6,11 @@
 // the forget gate), all in fp32:
 //     k_t = sigmoid(-forget_t),   g_t = span k_t
 //     h'_t = 0 where reset_t, else h_{t-1}
-//     h_t = g_t x_t + (h'_t - g_t h'_t)      (two fused steps; exactly x_t where g_t = 1)
+//     h_t = a_t h'_t + g_t x_t,  a_t = 1 - g_t
 //     y_t = h_t silu(z_t)                    (h_t without z)
 // k_t is 1 / (1 + e^forget): the complement of the gate is computed as such, so
 // that gates near one (long memory) keep their full relative precision.
-// Backward, with dh_t the gradient of h_t and a_t = 1 - g_t (0 at a reset):
+// Backward, with dh_t the gradient of h_t and a_t taken as 0 at a reset:
 //     dh_t = dy_t silu(z_t) + a_{t+1} dh_{t+1}   (+ dfinal at the last step)
 //     dx = g dh,  dg = dh (x - h'),  dforget = -dg g (1 - k),  dlower = -sum dg k
 //     dz = dy h silu'(z),  dinitial = a_0 dh_0
@@ -91,20 +91,19 @@ template <typename F> __device__ __forceinline__ F same(float v);
 template <> __device__ __forceinline__ float same<float>(float v) { return v; }
 template <> __device__ __forceinline__ float2 same<float2>(float v) { return f2(v); }
 template <typename F> __device__ __forceinline__ F sub(F a, F b) { return fm(b, same<F>(-1.0f), a); }
-template <typename F> __device__ __forceinline__ F neg(F a) { return mu(a, same<F>(-1.0f)); }
-template <typename F> __device__ __forceinline__ F step(F h, F g, F x) { return fm(g, x, fm(neg(g), h, h)); }
 
-// 2^v, with v limited to 120 so that 1 + 2^v stays finite (NaN passes).
-__device__ __forceinline__ float ex2_limited(float v) {
-    float m;
-    asm("min.NaN.f32 %0, %1, 0f42F00000;" : "=f"(m) : "f"(v));
-    return exp2_mufu(m);
-}
-// 1 / (1 + e^v): two MUFU operations.
-__device__ __forceinline__ float sigmoid_neg(float v) { return rcp_mufu(1.0f + ex2_limited(v * kLog2e)); }
+// 1 / (1 + e^v): two MUFU operations (e^v may overflow: the result is then 0).
+__device__ __forceinline__ float sigmoid_neg(float v) { return rcp_mufu(1.0f + exp2_mufu(v * kLog2e)); }
 __device__ __forceinline__ float2 sigmoid_neg(float2 v) {
     const float2 m = mul2(v, f2(kLog2e));
-    const float2 d = add2(f2(1.0f), make_float2(ex2_limited(m.x), ex2_limited(m.y)));
+    const float2 d = add2(f2(1.0f), make_float2(exp2_mufu(m.x), exp2_mufu(m.y)));
+    return make_float2(rcp_mufu(d.x), rcp_mufu(d.y));
+}
+// 1 / (1 + e^-v)
+__device__ __forceinline__ float sigmoid_pos(float v) { return rcp_mufu(1.0f + exp2_mufu(v * -kLog2e)); }
+__device__ __forceinline__ float2 sigmoid_pos(float2 v) {
+    const float2 m = mul2(v, f2(-kLog2e));
+    const float2 d = add2(f2(1.0f), make_float2(exp2_mufu(m.x), exp2_mufu(m.y)));
     return make_float2(rcp_mufu(d.x), rcp_mufu(d.y));
 }
 
@@ -122,6 +121,11 @@ template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) 
 template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+
+// A forget word whose gates keep the state (+infinity: g = 0), for steps past the end.
+template <typename T> constexpr uint32_t kKeep = 0x7f800000u;
+template <> constexpr uint32_t kKeep<__nv_bfloat16> = 0x7f807f80u;
+template <> constexpr uint32_t kKeep<__half> = 0x7c007c00u;
 
 // The lane's word at p: channels c (and c + 1) of `dim`; zero outside.
 template <typename T>
@@ -167,7 +171,6 @@ __device__ __forceinline__ void st_chan(float* p, int64_t c, int64_t dim, float2
 
 // Bit i: the i-th of the warp's steps (from t) is a reset.
 __device__ __forceinline__ uint32_t reset_mask(const uint8_t* reset, int64_t row, int64_t t, int64_t length) {
-    if (reset == nullptr) return 0u;
     const int lane = threadIdx.x & 31;
     const bool r = lane < kSteps && t + lane < length && reset[row + t + lane] != 0;
     return __ballot_sync(0xffffffffu, r);
@@ -221,7 +224,7 @@ template <typename F> __device__ __forceinline__ Map<F> then(const Map<F>& first
 // their chunks' maps through each other's shared memory, once a round.
 __device__ __forceinline__ int cluster_size() { return (int)cooperative_groups::this_cluster().num_blocks(); }
 
-template <typename T, bool GATE, bool TMA, int ST>
+template <typename T, bool GATE, bool RESET, bool TMA, int ST>
 __global__ void __launch_bounds__(kThreads, 3)
 fwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
@@ -244,18 +247,19 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
             for (int s = 0; s < ST && s < rounds; ++s)
                 ring.load(ta, s, (int)(tile * 32 * E), ((int64_t)s * C + rank) * kChunk, (int)b, which);
     }
-    F span, S;
+    F span, nspan, S;
     ld_chan(a.lower, c, a.dim, 0.0f, span);
+    nspan = sub(span, same<F>(1.0f));
     span = sub(same<F>(1.0f), span);
     ld_chan(a.init ? a.init + b * a.dim : nullptr, c, a.dim, 0.0f, S);
     for (int64_t n = 0; n < rounds; ++n) {
         const int64_t chunk = n * C + rank, t = chunk * kChunk + warp * kSteps;
         const int live = (int)max64(0, min64(kSteps, a.length - t));
-        uint32_t xw[kSteps], zw[kSteps];
-        F g[kSteps];
-        const uint32_t rs = reset_mask(a.reset, b * a.length, t, a.length);
+        uint32_t zw[kSteps];
+        F av[kSteps], bv[kSteps];                   // h -> av h + bv
+        const uint32_t rs = RESET ? reset_mask(a.reset, b * a.length, t, a.length) : 0u;
         {
-            uint32_t fw[kSteps];
+            uint32_t xw[kSteps], fw[kSteps];
             if constexpr (TMA) {
                 const int s = (int)(n % ST);
                 if (!tc::mbar_wait(ring.bar(s), (uint32_t)(n / ST) & 1u) && lane == 0) report(a, 111);
@@ -267,16 +271,23 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
                 ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
                 if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
             }
+            if (live < kSteps) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-                g[i] = i < live ? mu(span, sigmoid_neg(unpack<T>(fw[i]))) : same<F>(0.0f);
+                for (int i = 0; i < kSteps; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const F k = sigmoid_neg(unpack<T>(fw[i]));
+                av[i] = fm(nspan, k, same<F>(1.0f));
+                bv[i] = mu(mu(span, k), unpack<T>(xw[i]));
+            }
         }
         Map<F> m{same<F>(1.0f), same<F>(0.0f)};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            if (rs >> i & 1u) m = {same<F>(0.0f), same<F>(0.0f)};
-            m.H = step(m.H, g[i], unpack<T>(xw[i]));
-            m.A = fm(m.A, neg(g[i]), m.A);
+            if (RESET && (rs >> i & 1u)) m = {same<F>(0.0f), same<F>(0.0f)};
+            m.H = fm(av[i], m.H, bv[i]);
+            m.A = mu(m.A, av[i]);
         }
         Map<F>(*mw)[32] = maps[n & 1];
         mw[warp][lane] = m;
@@ -314,12 +325,12 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
         T* y = static_cast<T*>(a.y) + (b * a.length + t) * a.dim + c;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            if (rs >> i & 1u) h = same<F>(0.0f);
-            h = step(h, g[i], unpack<T>(xw[i]));
+            if (RESET && (rs >> i & 1u)) h = same<F>(0.0f);
+            h = fm(av[i], h, bv[i]);
             F o = h;
             if (GATE) {
                 const F z = unpack<T>(zw[i]);
-                o = mu(h, mu(z, sigmoid_neg(neg(z))));
+                o = mu(h, mu(z, sigmoid_pos(z)));
             }
             if (i < live) st_word<T>(y + i * a.dim, o, c, a.dim, a.words);
         }
@@ -327,7 +338,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     if (warp == 0 && rank == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
 }
 
-template <typename T, bool GATE, bool TMA, int ST>
+template <typename T, bool GATE, bool RESET, bool TMA, int ST>
 __global__ void __launch_bounds__(kThreads, 2)
 bwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
@@ -352,8 +363,9 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 ring.load(ta, s, (int)(tile * 32 * E), ((rounds - 1 - s) * C + rank) * kChunk, (int)b, which);
     }
     const F one = same<F>(1.0f), zero = same<F>(0.0f);
-    F span, D;
+    F span, nspan, D;
     ld_chan(a.lower, c, a.dim, 0.0f, span);
+    nspan = sub(span, one);
     span = sub(one, span);
     ld_chan(a.dfinal ? a.dfinal + b * a.dim : nullptr, c, a.dim, 0.0f, D);
     F dlower = zero;
@@ -362,7 +374,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         const int live = (int)max64(0, min64(kSteps, a.length - t));
         uint32_t xw[kSteps], zw[kSteps], dw[kSteps];
         F k[kSteps], h;
-        const uint32_t rs = reset_mask(a.reset, b * a.length, t, a.length);
+        const uint32_t rs = RESET ? reset_mask(a.reset, b * a.length, t, a.length) : 0u;
         ld_chan(chunk < a.chunks ? a.states + (b * a.chunks + chunk) * a.dim : nullptr, c, a.dim, 0.0f, h);
         {
             uint32_t fw[kSteps];
@@ -379,16 +391,20 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
                 ld_steps<T>(a.dy, b * a.dyb, a.dyt, t, live, c, a, dw);
             }
+            if (live < kSteps) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) k[i] = i < live ? sigmoid_neg(unpack<T>(fw[i])) : zero;
+                for (int i = 0; i < kSteps; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) k[i] = sigmoid_neg(unpack<T>(fw[i]));
         }
         Map<F> m{one, zero};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const F g = mu(span, k[i]);
-            if (rs >> i & 1u) m = {zero, zero};
-            m.H = step(m.H, g, unpack<T>(xw[i]));
-            m.A = fm(m.A, neg(g), m.A);
+            const F av = fm(nspan, k[i], one);
+            if (RESET && (rs >> i & 1u)) m = {zero, zero};
+            m.H = fm(av, m.H, mu(mu(span, k[i]), unpack<T>(xw[i])));
+            m.A = mu(m.A, av);
         }
         F d = zero;
 #pragma unroll
@@ -396,11 +412,10 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
             F e = unpack<T>(dw[i]);
             if (GATE) {
                 const F z = unpack<T>(zw[i]);
-                e = mu(e, mu(z, sigmoid_neg(neg(z))));
+                e = mu(e, mu(z, sigmoid_pos(z)));
             }
-            d = ad(d, e);
-            d = fm(d, neg(mu(span, k[i])), d);
-            if (rs >> i & 1u) d = zero;
+            d = mu(ad(d, e), fm(nspan, k[i], one));
+            if (RESET && (rs >> i & 1u)) d = zero;
         }
         auto& mw = maps[turn & 1];
         mw[warp].m[lane] = m;
@@ -439,23 +454,23 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         F hp[kSteps];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            if (rs >> i & 1u) h = zero;
+            if (RESET && (rs >> i & 1u)) h = zero;
             hp[i] = h;
-            h = step(h, mu(span, k[i]), unpack<T>(xw[i]));
+            h = fm(fm(nspan, k[i], one), h, mu(mu(span, k[i]), unpack<T>(xw[i])));
         }
         const int64_t at = (b * a.length + t) * a.dim + c;
         F dl = zero;
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
-            const F g = mu(span, k[i]), x = unpack<T>(xw[i]), dy = unpack<T>(dw[i]);
+            const F g = mu(span, k[i]), av = fm(nspan, k[i], one), x = unpack<T>(xw[i]), dy = unpack<T>(dw[i]);
             F e = dy;
             if (GATE) {
-                const F z = unpack<T>(zw[i]), s = sigmoid_neg(neg(z)), zs = mu(z, s);
+                const F z = unpack<T>(zw[i]), s = sigmoid_pos(z), zs = mu(z, s);
                 e = mu(dy, zs);
                 // silu'(z) = s + z s (1 - s)
                 const F ds = fm(zs, sub(one, s), s);
                 if (i < live)
-                    st_word<T>(static_cast<T*>(a.dz) + at + i * a.dim, mu(mu(dy, step(hp[i], g, x)), ds), c, a.dim,
+                    st_word<T>(static_cast<T*>(a.dz) + at + i * a.dim, mu(mu(dy, fm(av, hp[i], mu(g, x))), ds), c, a.dim,
                                a.words);
             }
             d = ad(d, e);                          // dh of step i
@@ -466,8 +481,8 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                            a.words);
             }
             dl = fm(dg, k[i], dl);
-            d = fm(d, neg(g), d);
-            if (rs >> i & 1u) d = zero;
+            d = mu(d, av);
+            if (RESET && (rs >> i & 1u)) d = zero;
         }
         dlower = sub(dlower, dl);
     }
@@ -515,9 +530,9 @@ step_kernel(const StepArgs a) {
     ld_chan(a.lower, c, a.dim, 0.0f, span);
     ld_chan(a.state + b * a.sb, c, a.dim, 0.0f, h);
     const F g = mu(sub(same<F>(1.0f), span), sigmoid_neg(f));
-    h = step(h, g, x);
+    h = fm(sub(same<F>(1.0f), g), h, mu(g, x));
     st_chan(a.state + b * a.sb, c, a.dim, h);
-    if (GATE) h = mu(h, mu(z, sigmoid_neg(neg(z))));
+    if (GATE) h = mu(h, mu(z, sigmoid_pos(z)));
     st_word<T>(static_cast<T*>(a.y) + b * a.dim + c, h, c, a.dim, a.words);
 }
 
@@ -641,23 +656,25 @@ static int launch_kernel(K kernel, const TmaArgs& ta, unsigned tiles, int cluste
 
 constexpr int kFwdStages = 2, kBwdStages = 2;
 
-template <typename T, bool GATE>
+template <typename T, bool GATE, bool RESET>
 static int launch(const TmaArgs& ta, bool bwd, bool tma, int cluster, cudaStream_t st) {
     const unsigned tiles = (unsigned)ceil_div(ta.a.dim, 32 * Lane<T>::E);
     constexpr size_t fs = Ring<GATE ? 3 : 2, kFwdStages>::bytes, bs = Ring<GATE ? 4 : 3, kBwdStages>::bytes;
     if (bwd) {
         const char* what = "gated_linear_recurrence bwd";
-        if (tma) return launch_kernel(bwd_kernel<T, GATE, true, kBwdStages>, ta, tiles, cluster, bs, st, what);
-        return launch_kernel(bwd_kernel<T, GATE, false, kBwdStages>, ta, tiles, cluster, 0, st, what);
+        if (tma) return launch_kernel(bwd_kernel<T, GATE, RESET, true, kBwdStages>, ta, tiles, cluster, bs, st, what);
+        return launch_kernel(bwd_kernel<T, GATE, RESET, false, kBwdStages>, ta, tiles, cluster, 0, st, what);
     }
     const char* what = "gated_linear_recurrence fwd";
-    if (tma) return launch_kernel(fwd_kernel<T, GATE, true, kFwdStages>, ta, tiles, cluster, fs, st, what);
-    return launch_kernel(fwd_kernel<T, GATE, false, kFwdStages>, ta, tiles, cluster, 0, st, what);
+    if (tma) return launch_kernel(fwd_kernel<T, GATE, RESET, true, kFwdStages>, ta, tiles, cluster, fs, st, what);
+    return launch_kernel(fwd_kernel<T, GATE, RESET, false, kFwdStages>, ta, tiles, cluster, 0, st, what);
 }
 
 template <typename T>
 static int launch_gate(const TmaArgs& ta, bool bwd, bool tma, int cluster, cudaStream_t st) {
-    return ta.a.z ? launch<T, true>(ta, bwd, tma, cluster, st) : launch<T, false>(ta, bwd, tma, cluster, st);
+    if (ta.a.reset)
+        return ta.a.z ? launch<T, true, true>(ta, bwd, tma, cluster, st) : launch<T, false, true>(ta, bwd, tma, cluster, st);
+    return ta.a.z ? launch<T, true, false>(ta, bwd, tma, cluster, st) : launch<T, false, false>(ta, bwd, tma, cluster, st);
 }
 
 static int launch_any(const ssm_gated_recurrence_params* p, const Args& a, bool bwd, cudaStream_t st) {
