@@ -215,6 +215,21 @@ struct Ring {
     }
 };
 
+// The values as the compiler cannot know them: what is computed from them later is
+// computed again rather than kept in registers from an earlier use.
+__device__ __forceinline__ void again(uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+r"(w[i]));
+}
+__device__ __forceinline__ void again(float* v) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void again(float2* v) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+f"(v[i].x), "+f"(v[i].y));
+}
+
 template <typename F> struct Map { F A, H; };
 template <typename F> __device__ __forceinline__ Map<F> then(const Map<F>& first, const Map<F>& next) {
     return {mu(first.A, next.A), through(next.A, next.H, first.H)};
@@ -451,6 +466,8 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
             const Map<F> o = mw[w].m[lane];
             h = through(o.A, o.H, h);
         }
+        again(xw);
+        again(k);
         F hp[kSteps];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -458,6 +475,10 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
             hp[i] = h;
             h = fm(fm(nspan, k[i], one), h, mu(mu(span, k[i]), unpack<T>(xw[i])));
         }
+        again(xw);
+        again(k);
+        again(dw);
+        if (GATE) again(zw);
         const int64_t at = (b * a.length + t) * a.dim + c;
         F dl = zero;
 #pragma unroll
