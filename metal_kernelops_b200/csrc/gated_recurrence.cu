@@ -17,7 +17,7 @@
 //
 // Both directions are scans of affine maps: a run of steps takes the state S to
 // A S + H, with A the product of the a_t, and the gradient D that enters it from
-// the later steps to A D + R.  A warp owns kSteps consecutive steps of a tile of
+// the later steps to A D + R.  A warp owns N consecutive steps of a tile of
 // channels (a lane: one 4-byte word, two 16-bit channels or one fp32 channel),
 // holds them in registers, and reduces them to (A, H); the warps' maps meet in
 // shared memory, each warp composes those before it and walks its steps a second
@@ -46,12 +46,13 @@ namespace ssm {
 namespace glr {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kSteps = 8, kChunk = kWarps * kSteps;
-constexpr int kTile = kChunk * 128;                 // bytes of one tensor's chunk: 128-byte rows
+constexpr int kFwdSteps = 16, kBwdSteps = 8;         // a warp's steps of a chunk
 constexpr int kMaxCluster = 8;
+constexpr int kRow = 128;                           // bytes of a step of one tensor
 
 struct Args {
-    int64_t batch, length, dim, chunks;
+    int64_t batch, length, dim, chunks;             // chunks of this pass
+    int64_t saved;                                  // states saved per batch row (every kBwdSteps kWarps steps)
     int64_t xt, xb, ft, fb, zt, zb, dyt, dyb;      // token and batch strides
     const void* x; const void* forget; const void* z;
     const float* lower; const float* init; const uint8_t* reset;
@@ -107,10 +108,15 @@ __device__ __forceinline__ float2 sigmoid_pos(float2 v) {
     return make_float2(rcp_mufu(d.x), rcp_mufu(d.y));
 }
 
-// S -> A S + H; where A is 0 the state that enters does not matter.
-__device__ __forceinline__ float through(float A, float H, float S) { return A == 0.0f ? H : fmaf(A, S, H); }
+// S -> A S + H; with resets, where A is 0 the state that enters does not matter.
+template <bool RESET>
+__device__ __forceinline__ float through(float A, float H, float S) {
+    return RESET && A == 0.0f ? H : fmaf(A, S, H);
+}
+template <bool RESET>
 __device__ __forceinline__ float2 through(float2 A, float2 H, float2 S) {
-    return make_float2(through(A.x, H.x, S.x), through(A.y, H.y, S.y));
+    if constexpr (!RESET) return fma2(A, S, H);
+    return make_float2(through<true>(A.x, H.x, S.x), through<true>(A.y, H.y, S.y));
 }
 
 template <typename T> __device__ __forceinline__ typename Lane<T>::F unpack(uint32_t w);
@@ -140,6 +146,8 @@ __device__ __forceinline__ uint32_t ld_word(const T* p, int64_t c, int64_t dim, 
         return w;
     }
 }
+__device__ __forceinline__ void st_lane(float* p, float v) { *p = v; }
+template <typename T> __device__ __forceinline__ void st_lane(T* p, float2 v) { Io2<T>::st(p, v); }
 template <typename T>
 __device__ __forceinline__ void st_word(T* p, typename Lane<T>::F v, int64_t c, int64_t dim, bool words) {
     if constexpr (sizeof(T) == 4) {
@@ -169,26 +177,28 @@ __device__ __forceinline__ void st_chan(float* p, int64_t c, int64_t dim, float2
     if (c + 1 < dim) p[c + 1] = v.y;
 }
 
-// Bit i: the i-th of the warp's steps (from t) is a reset.
+// Bit i: the i-th of the warp's N steps (from t) is a reset.
+template <int N>
 __device__ __forceinline__ uint32_t reset_mask(const uint8_t* reset, int64_t row, int64_t t, int64_t length) {
     const int lane = threadIdx.x & 31;
-    const bool r = lane < kSteps && t + lane < length && reset[row + t + lane] != 0;
+    const bool r = lane < N && t + lane < length && reset[row + t + lane] != 0;
     return __ballot_sync(0xffffffffu, r);
 }
 
-template <typename T>
-__device__ __forceinline__ void ld_steps(const void* base, int64_t row, int64_t stride, int64_t t, int n, int64_t c,
+template <typename T, int N>
+__device__ __forceinline__ void ld_steps(const void* base, int64_t row, int64_t stride, int64_t t, int live, int64_t c,
                                          const Args& a, uint32_t* w) {
     const T* p = static_cast<const T*>(base) + row + t * stride + c;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) w[i] = i < n ? ld_word<T>(p + i * stride, c, a.dim, a.words) : 0u;
+    for (int i = 0; i < N; ++i) w[i] = i < live ? ld_word<T>(p + i * stride, c, a.dim, a.words) : 0u;
 }
 
 // The ring of chunk tiles in shared memory that TMA fills: stage s holds NT
-// tensors' chunks, a warp's steps being kSteps consecutive 128-byte rows of each.
+// tensors' chunks, a warp's steps being N consecutive 128-byte rows of each.
 // Thread 0 issues; the wait of a stage is every thread's.
-template <int NT, int ST>
+template <int NT, int ST, int N>
 struct Ring {
+    static constexpr int kTile = kWarps * N * kRow;   // bytes of one tensor's chunk
     uint8_t* base;                  // ST * NT * kTile bytes, then ST mbarriers
     static constexpr size_t bytes = (size_t)ST * NT * kTile + ST * 8;
     __device__ __forceinline__ uint32_t bar(int s) const {
@@ -208,47 +218,51 @@ struct Ring {
             tc::tma_load3(tc::smem_u32(base + (s * NT + i) * kTile), &ta.m[which[i]], c0, (int)t, b, bar(s));
     }
     __device__ __forceinline__ void read(int s, int i, uint32_t* w) const {
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (s * NT + i) * kTile) + threadIdx.x / 32 * kSteps * 32 +
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (s * NT + i) * kTile) + threadIdx.x / 32 * N * 32 +
                             (threadIdx.x & 31);
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) w[k] = p[k * 32];
+        for (int k = 0; k < N; ++k) w[k] = p[k * 32];
     }
 };
 
 // The values as the compiler cannot know them: what is computed from them later is
 // computed again rather than kept in registers from an earlier use.
-__device__ __forceinline__ void again(uint32_t* w) {
+template <int N>
+__device__ __forceinline__ void again(uint32_t (&w)[N]) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+r"(w[i]));
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(w[i]));
 }
-__device__ __forceinline__ void again(float* v) {
+template <int N>
+__device__ __forceinline__ void again(float (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+f"(v[i]));
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
-__device__ __forceinline__ void again(float2* v) {
+template <int N>
+__device__ __forceinline__ void again(float2 (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+f"(v[i].x), "+f"(v[i].y));
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i].x), "+f"(v[i].y));
 }
 
 template <typename F> struct Map { F A, H; };
-template <typename F> __device__ __forceinline__ Map<F> then(const Map<F>& first, const Map<F>& next) {
-    return {mu(first.A, next.A), through(next.A, next.H, first.H)};
+template <bool RESET, typename F>
+__device__ __forceinline__ Map<F> then(const Map<F>& first, const Map<F>& next) {
+    return {mu(first.A, next.A), through<RESET>(next.A, next.H, first.H)};
 }
 
 // A cluster of C CTAs takes C consecutive chunks at a time: its CTAs exchange
 // their chunks' maps through each other's shared memory, once a round.
 __device__ __forceinline__ int cluster_size() { return (int)cooperative_groups::this_cluster().num_blocks(); }
 
-template <typename T, bool GATE, bool RESET, bool TMA, int ST>
-__global__ void __launch_bounds__(kThreads, 3)
+template <typename T, bool GATE, bool RESET, bool TMA, int ST, int N>
+__global__ void __launch_bounds__(kThreads, N > 8 ? 2 : 3)
 fwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
-    constexpr int E = Lane<T>::E, NT = GATE ? 3 : 2;
+    constexpr int E = Lane<T>::E, NT = GATE ? 3 : 2, kChunk = kWarps * N;
     const Args& a = ta.a;
     __shared__ Map<F> maps[2][kWarps][32];
     __shared__ Map<F> far[2][kMaxCluster][32];
     extern __shared__ __align__(128) uint8_t smem[];
-    const Ring<NT, ST> ring{smem};
+    const Ring<NT, ST, N> ring{smem};
     const int which[3] = {0, 1, 2};
     const auto cluster = cooperative_groups::this_cluster();
     const int C = cluster_size(), rank = (int)cluster.block_rank();
@@ -268,13 +282,13 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     span = sub(same<F>(1.0f), span);
     ld_chan(a.init ? a.init + b * a.dim : nullptr, c, a.dim, 0.0f, S);
     for (int64_t n = 0; n < rounds; ++n) {
-        const int64_t chunk = n * C + rank, t = chunk * kChunk + warp * kSteps;
-        const int live = (int)max64(0, min64(kSteps, a.length - t));
-        uint32_t zw[kSteps];
-        F av[kSteps], bv[kSteps];                   // h -> av h + bv
-        const uint32_t rs = RESET ? reset_mask(a.reset, b * a.length, t, a.length) : 0u;
+        const int64_t chunk = n * C + rank, t = chunk * kChunk + warp * N;
+        const int live = (int)max64(0, min64(N, a.length - t));
+        uint32_t zw[N];
+        F av[N], bv[N];                   // h -> av h + bv
+        const uint32_t rs = RESET ? reset_mask<N>(a.reset, b * a.length, t, a.length) : 0u;
         {
-            uint32_t xw[kSteps], fw[kSteps];
+            uint32_t xw[N], fw[N];
             if constexpr (TMA) {
                 const int s = (int)(n % ST);
                 if (!tc::mbar_wait(ring.bar(s), (uint32_t)(n / ST) & 1u) && lane == 0) report(a, 111);
@@ -282,16 +296,16 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
                 ring.read(s, 1, fw);
                 if (GATE) ring.read(s, 2, zw);
             } else {
-                ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
-                ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
-                if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
+                ld_steps<T, N>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
+                ld_steps<T, N>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
+                if (GATE) ld_steps<T, N>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
             }
-            if (live < kSteps) {
+            if (live < N) {
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
+                for (int i = 0; i < N; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
             }
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
+            for (int i = 0; i < N; ++i) {
                 const F k = sigmoid_neg(unpack<T>(fw[i]));
                 av[i] = fm(nspan, k, same<F>(1.0f));
                 bv[i] = mu(mu(span, k), unpack<T>(xw[i]));
@@ -299,7 +313,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
         }
         Map<F> m{same<F>(1.0f), same<F>(0.0f)};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        for (int i = 0; i < N; ++i) {
             if (RESET && (rs >> i & 1u)) m = {same<F>(0.0f), same<F>(0.0f)};
             m.H = fm(av[i], m.H, bv[i]);
             m.A = mu(m.A, av[i]);
@@ -312,34 +326,35 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
             ring.load(ta, (int)(n % ST), (int)(tile * 32 * E), ((n + ST) * C + rank) * kChunk, (int)b, which);
         F h;
         if (C == 1) {
-            if (a.states != nullptr && warp == 0) st_chan(a.states + (b * a.chunks + chunk) * a.dim, c, a.dim, S);
             h = S;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const Map<F> o = mw[w][lane];
                 if (w == warp) h = S;
-                S = through(o.A, o.H, S);
+                S = through<RESET>(o.A, o.H, S);
             }
         } else {
             Map<F> before{same<F>(1.0f), same<F>(0.0f)};
-            for (int w = 0; w < warp; ++w) before = then(before, mw[w][lane]);
+            for (int w = 0; w < warp; ++w) before = then<RESET>(before, mw[w][lane]);
             if (warp == kWarps - 1) {
-                const Map<F> all = then(before, m);
+                const Map<F> all = then<RESET>(before, m);
                 for (int r = 0; r < C; ++r) cluster.map_shared_rank(&far[n & 1][0][0], r)[rank * 32 + lane] = all;
             }
             cluster.sync();
             for (int r = 0; r < C; ++r) {
                 if (r == rank) h = S;
                 const Map<F> o = far[n & 1][r][lane];
-                S = through(o.A, o.H, S);
+                S = through<RESET>(o.A, o.H, S);
             }
-            if (a.states != nullptr && warp == 0 && chunk < a.chunks)
-                st_chan(a.states + (b * a.chunks + chunk) * a.dim, c, a.dim, h);
-            h = through(before.A, before.H, h);
+            h = through<RESET>(before.A, before.H, h);
         }
+        // the state that enters every kBwdSteps kWarps steps, for the backward
+        if (a.states != nullptr && warp % (kBwdSteps * kWarps / N) == 0 && live > 0)
+            st_chan(a.states + (b * a.saved + t / (kBwdSteps * kWarps)) * a.dim, c, a.dim, h);
         T* y = static_cast<T*>(a.y) + (b * a.length + t) * a.dim + c;
+        const bool whole = live == N && a.words && c + E <= a.dim;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        for (int i = 0; i < N; ++i) {
             if (RESET && (rs >> i & 1u)) h = same<F>(0.0f);
             h = fm(av[i], h, bv[i]);
             F o = h;
@@ -347,23 +362,24 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
                 const F z = unpack<T>(zw[i]);
                 o = mu(h, mu(z, sigmoid_pos(z)));
             }
-            if (i < live) st_word<T>(y + i * a.dim, o, c, a.dim, a.words);
+            if (whole) st_lane(y + i * a.dim, o);
+            else if (i < live) st_word<T>(y + i * a.dim, o, c, a.dim, a.words);
         }
     }
     if (warp == 0 && rank == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
 }
 
-template <typename T, bool GATE, bool RESET, bool TMA, int ST>
+template <typename T, bool GATE, bool RESET, bool TMA, int ST, int N>
 __global__ void __launch_bounds__(kThreads, 2)
 bwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
-    constexpr int E = Lane<T>::E, NT = GATE ? 4 : 3;
+    constexpr int E = Lane<T>::E, NT = GATE ? 4 : 3, kChunk = kWarps * N;
     const Args& a = ta.a;
     __shared__ struct { Map<F> m[32]; F R[32]; } maps[2][kWarps];
     __shared__ Map<F> far[2][kMaxCluster][32];          // H holds R here
     __shared__ F sums[kWarps][32];
     extern __shared__ __align__(128) uint8_t smem[];
-    const Ring<NT, ST> ring{smem};
+    const Ring<NT, ST, N> ring{smem};
     const int which[4] = {0, 1, 3, 2};                  // x, forget, dy, z
     const auto cluster = cooperative_groups::this_cluster();
     const int C = cluster_size(), rank = (int)cluster.block_rank();
@@ -385,14 +401,14 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
     ld_chan(a.dfinal ? a.dfinal + b * a.dim : nullptr, c, a.dim, 0.0f, D);
     F dlower = zero;
     for (int64_t turn = 0; turn < rounds; ++turn) {
-        const int64_t chunk = (rounds - 1 - turn) * C + rank, t = chunk * kChunk + warp * kSteps;
-        const int live = (int)max64(0, min64(kSteps, a.length - t));
-        uint32_t xw[kSteps], zw[kSteps], dw[kSteps];
-        F k[kSteps], h;
-        const uint32_t rs = RESET ? reset_mask(a.reset, b * a.length, t, a.length) : 0u;
-        ld_chan(chunk < a.chunks ? a.states + (b * a.chunks + chunk) * a.dim : nullptr, c, a.dim, 0.0f, h);
+        const int64_t chunk = (rounds - 1 - turn) * C + rank, t = chunk * kChunk + warp * N;
+        const int live = (int)max64(0, min64(N, a.length - t));
+        uint32_t xw[N], zw[N], dw[N];
+        F k[N], h;
+        const uint32_t rs = RESET ? reset_mask<N>(a.reset, b * a.length, t, a.length) : 0u;
+        ld_chan(chunk < a.chunks ? a.states + (b * a.saved + chunk) * a.dim : nullptr, c, a.dim, 0.0f, h);
         {
-            uint32_t fw[kSteps];
+            uint32_t fw[N];
             if constexpr (TMA) {
                 const int s = (int)(turn % ST);
                 if (!tc::mbar_wait(ring.bar(s), (uint32_t)(turn / ST) & 1u) && lane == 0) report(a, 112);
@@ -401,21 +417,21 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 ring.read(s, 2, dw);
                 if (GATE) ring.read(s, 3, zw);
             } else {
-                ld_steps<T>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
-                ld_steps<T>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
-                if (GATE) ld_steps<T>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
-                ld_steps<T>(a.dy, b * a.dyb, a.dyt, t, live, c, a, dw);
+                ld_steps<T, N>(a.x, b * a.xb, a.xt, t, live, c, a, xw);
+                ld_steps<T, N>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
+                if (GATE) ld_steps<T, N>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
+                ld_steps<T, N>(a.dy, b * a.dyb, a.dyt, t, live, c, a, dw);
             }
-            if (live < kSteps) {
+            if (live < N) {
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
+                for (int i = 0; i < N; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
             }
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) k[i] = sigmoid_neg(unpack<T>(fw[i]));
+            for (int i = 0; i < N; ++i) k[i] = sigmoid_neg(unpack<T>(fw[i]));
         }
         Map<F> m{one, zero};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        for (int i = 0; i < N; ++i) {
             const F av = fm(nspan, k[i], one);
             if (RESET && (rs >> i & 1u)) m = {zero, zero};
             m.H = fm(av, m.H, mu(mu(span, k[i]), unpack<T>(xw[i])));
@@ -423,7 +439,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         }
         F d = zero;
 #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i) {
+        for (int i = N - 1; i >= 0; --i) {
             F e = unpack<T>(dw[i]);
             if (GATE) {
                 const F z = unpack<T>(zw[i]);
@@ -445,32 +461,32 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
             for (int w = kWarps - 1; w >= 0; --w) {
                 const F A = mw[w].m[lane].A;
                 if (w == warp) d = D;
-                D = through(A, mw[w].R[lane], D);
+                D = through<RESET>(A, mw[w].R[lane], D);
             }
         } else {
             Map<F> after{one, zero};
-            for (int w = kWarps - 1; w > warp; --w) after = then(after, Map<F>{mw[w].m[lane].A, mw[w].R[lane]});
+            for (int w = kWarps - 1; w > warp; --w) after = then<RESET>(after, Map<F>{mw[w].m[lane].A, mw[w].R[lane]});
             if (warp == 0) {
-                const Map<F> all = then(after, Map<F>{m.A, d});
+                const Map<F> all = then<RESET>(after, Map<F>{m.A, d});
                 for (int r = 0; r < C; ++r) cluster.map_shared_rank(&far[turn & 1][0][0], r)[rank * 32 + lane] = all;
             }
             cluster.sync();
             for (int r = C - 1; r >= 0; --r) {
                 if (r == rank) d = D;
                 const Map<F> o = far[turn & 1][r][lane];
-                D = through(o.A, o.H, D);
+                D = through<RESET>(o.A, o.H, D);
             }
-            d = through(after.A, after.H, d);
+            d = through<RESET>(after.A, after.H, d);
         }
         for (int w = 0; w < warp; ++w) {
             const Map<F> o = mw[w].m[lane];
-            h = through(o.A, o.H, h);
+            h = through<RESET>(o.A, o.H, h);
         }
         again(xw);
         again(k);
-        F hp[kSteps];
+        F hp[N];
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        for (int i = 0; i < N; ++i) {
             if (RESET && (rs >> i & 1u)) h = zero;
             hp[i] = h;
             h = fm(fm(nspan, k[i], one), h, mu(mu(span, k[i]), unpack<T>(xw[i])));
@@ -480,9 +496,15 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         again(dw);
         if (GATE) again(zw);
         const int64_t at = (b * a.length + t) * a.dim + c;
+        const bool whole = live == N && a.words && c + E <= a.dim;
+        auto put = [&](void* base, int i, F v) {
+            T* p = static_cast<T*>(base) + at + i * a.dim;
+            if (whole) st_lane(p, v);
+            else if (i < live) st_word<T>(p, v, c, a.dim, a.words);
+        };
         F dl = zero;
 #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i) {
+        for (int i = N - 1; i >= 0; --i) {
             const F g = mu(span, k[i]), av = fm(nspan, k[i], one), x = unpack<T>(xw[i]), dy = unpack<T>(dw[i]);
             F e = dy;
             if (GATE) {
@@ -490,17 +512,12 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 e = mu(dy, zs);
                 // silu'(z) = s + z s (1 - s)
                 const F ds = fm(zs, sub(one, s), s);
-                if (i < live)
-                    st_word<T>(static_cast<T*>(a.dz) + at + i * a.dim, mu(mu(dy, fm(av, hp[i], mu(g, x))), ds), c, a.dim,
-                               a.words);
+                put(a.dz, i, mu(mu(dy, fm(av, hp[i], mu(g, x))), ds));
             }
             d = ad(d, e);                          // dh of step i
             const F dg = mu(d, sub(x, hp[i]));
-            if (i < live) {
-                st_word<T>(static_cast<T*>(a.dx) + at + i * a.dim, mu(g, d), c, a.dim, a.words);
-                st_word<T>(static_cast<T*>(a.dforget) + at + i * a.dim, mu(mu(dg, g), sub(k[i], one)), c, a.dim,
-                           a.words);
-            }
+            put(a.dx, i, mu(g, d));
+            put(a.dforget, i, mu(mu(dg, g), sub(k[i], one)));
             dl = fm(dg, k[i], dl);
             d = mu(d, av);
             if (RESET && (rs >> i & 1u)) d = zero;
@@ -573,10 +590,11 @@ static int validate(const ssm_gated_recurrence_params* p) {
     return SSM_OK;
 }
 
-static Args args_of(const ssm_gated_recurrence_params* p) {
+static Args args_of(const ssm_gated_recurrence_params* p, bool bwd) {
     Args a{};
     a.batch = p->batch; a.length = p->length; a.dim = p->dim;
-    a.chunks = ceil_div(p->length, kChunk);
+    a.chunks = ceil_div(p->length, kWarps * (bwd ? kBwdSteps : kFwdSteps));
+    a.saved = ceil_div(p->length, kWarps * kBwdSteps);
     auto token = [&](int64_t s) { return s ? s : p->dim; };
     auto row = [&](int64_t s, int64_t t) { return s ? s : t * p->length; };
     a.xt = token(p->x_token_stride); a.xb = row(p->x_batch_stride, a.xt);
@@ -617,12 +635,12 @@ static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 }
 
 // (batch, length, dim) as (channel, token, batch row); box: one chunk of 128-byte rows.
-static int encode(CUtensorMap* m, const void* base, int64_t token, int64_t row, int dtype, const Args& a) {
+static int encode(CUtensorMap* m, const void* base, int64_t token, int64_t row, int dtype, int chunk, const Args& a) {
     const int64_t es = esize(dtype);
     cuuint64_t dims[3] = {(cuuint64_t)a.dim, (cuuint64_t)a.length, (cuuint64_t)a.batch};
     // a single row's stride is never used, but has to be a valid one
     cuuint64_t strides[2] = {(cuuint64_t)(token * es), (cuuint64_t)((a.batch > 1 ? row : token) * es)};
-    cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)kChunk, 1};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)chunk, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     const CUtensorMapDataType type = dtype == SSM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : dtype == SSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -648,8 +666,9 @@ static bool tma_ok(const Args& a, int dtype, bool bwd) {
 
 // CTAs of a cluster: as many (a power of two, up to 8, no more than chunks) as
 // bring the grid to two CTAs per SM.
-static int cluster_of(const ssm_gated_recurrence_params* p) {
-    const int64_t tiles = ceil_div(p->dim * esize(p->dtype), 128), chunks = ceil_div(p->length, kChunk);
+static int cluster_of(const ssm_gated_recurrence_params* p, bool bwd) {
+    const int64_t tiles = ceil_div(p->dim * esize(p->dtype), kRow);
+    const int64_t chunks = ceil_div(p->length, kWarps * (bwd ? kBwdSteps : kFwdSteps));
     int c = 1;
     while (c < kMaxCluster && 2 * c <= chunks && tiles * p->batch * c < 148 * 2) c *= 2;
     return c;
@@ -680,15 +699,16 @@ constexpr int kFwdStages = 2, kBwdStages = 2;
 template <typename T, bool GATE, bool RESET>
 static int launch(const TmaArgs& ta, bool bwd, bool tma, int cluster, cudaStream_t st) {
     const unsigned tiles = (unsigned)ceil_div(ta.a.dim, 32 * Lane<T>::E);
-    constexpr size_t fs = Ring<GATE ? 3 : 2, kFwdStages>::bytes, bs = Ring<GATE ? 4 : 3, kBwdStages>::bytes;
+    constexpr size_t fs = Ring<GATE ? 3 : 2, kFwdStages, kFwdSteps>::bytes,
+                     bs = Ring<GATE ? 4 : 3, kBwdStages, kBwdSteps>::bytes;
     if (bwd) {
         const char* what = "gated_linear_recurrence bwd";
-        if (tma) return launch_kernel(bwd_kernel<T, GATE, RESET, true, kBwdStages>, ta, tiles, cluster, bs, st, what);
-        return launch_kernel(bwd_kernel<T, GATE, RESET, false, kBwdStages>, ta, tiles, cluster, 0, st, what);
+        if (tma) return launch_kernel(bwd_kernel<T, GATE, RESET, true, kBwdStages, kBwdSteps>, ta, tiles, cluster, bs, st, what);
+        return launch_kernel(bwd_kernel<T, GATE, RESET, false, kBwdStages, kBwdSteps>, ta, tiles, cluster, 0, st, what);
     }
     const char* what = "gated_linear_recurrence fwd";
-    if (tma) return launch_kernel(fwd_kernel<T, GATE, RESET, true, kFwdStages>, ta, tiles, cluster, fs, st, what);
-    return launch_kernel(fwd_kernel<T, GATE, RESET, false, kFwdStages>, ta, tiles, cluster, 0, st, what);
+    if (tma) return launch_kernel(fwd_kernel<T, GATE, RESET, true, kFwdStages, kFwdSteps>, ta, tiles, cluster, fs, st, what);
+    return launch_kernel(fwd_kernel<T, GATE, RESET, false, kFwdStages, kFwdSteps>, ta, tiles, cluster, 0, st, what);
 }
 
 template <typename T>
@@ -702,16 +722,17 @@ static int launch_any(const ssm_gated_recurrence_params* p, const Args& a, bool 
     TmaArgs ta{};
     ta.a = a;
     const bool tma = tma_ok(a, p->dtype, bwd);
+    const int chunk = kWarps * (bwd ? kBwdSteps : kFwdSteps);
     if (tma) {
         if (int s = ensure_context("gated_linear_recurrence")) return s;
-        if (int s = encode(&ta.m[0], a.x, a.xt, a.xb, p->dtype, a)) return s;
-        if (int s = encode(&ta.m[1], a.forget, a.ft, a.fb, p->dtype, a)) return s;
+        if (int s = encode(&ta.m[0], a.x, a.xt, a.xb, p->dtype, chunk, a)) return s;
+        if (int s = encode(&ta.m[1], a.forget, a.ft, a.fb, p->dtype, chunk, a)) return s;
         if (a.z)
-            if (int s = encode(&ta.m[2], a.z, a.zt, a.zb, p->dtype, a)) return s;
+            if (int s = encode(&ta.m[2], a.z, a.zt, a.zb, p->dtype, chunk, a)) return s;
         if (bwd)
-            if (int s = encode(&ta.m[3], a.dy, a.dyt, a.dyb, p->dtype, a)) return s;
+            if (int s = encode(&ta.m[3], a.dy, a.dyt, a.dyb, p->dtype, chunk, a)) return s;
     }
-    const int cluster = cluster_of(p);
+    const int cluster = cluster_of(p, bwd);
     if (p->dtype == SSM_F32) return launch_gate<float>(ta, bwd, tma, cluster, st);
     if (p->dtype == SSM_BF16) return launch_gate<__nv_bfloat16>(ta, bwd, tma, cluster, st);
     return launch_gate<__half>(ta, bwd, tma, cluster, st);
@@ -745,8 +766,8 @@ int ssm_glr_take_error() {
 extern "C" int ssm_gated_recurrence_sizes(const ssm_gated_recurrence_params* p, size_t* states_bytes,
                                           size_t* workspace_bytes) {
     if (int s = validate(p)) return s;
-    if (states_bytes) *states_bytes = (size_t)(p->batch * ceil_div(p->length, kChunk) * p->dim) * 4;
-    if (workspace_bytes) *workspace_bytes = (size_t)(p->batch * cluster_of(p) * p->dim) * 4;
+    if (states_bytes) *states_bytes = (size_t)(p->batch * ceil_div(p->length, kWarps * kBwdSteps) * p->dim) * 4;
+    if (workspace_bytes) *workspace_bytes = (size_t)(p->batch * cluster_of(p, true) * p->dim) * 4;
     return SSM_OK;
 }
 
@@ -755,7 +776,7 @@ extern "C" int ssm_gated_recurrence_fwd(const ssm_gated_recurrence_params* p, vo
     if (p->batch == 0) return SSM_OK;
     if (!p->final_state || (p->length && (!p->x || !p->forget || !p->y)))
         return fail(SSM_ERR_INVALID, "gated_linear_recurrence fwd: null pointer");
-    return launch_any(p, args_of(p), false, static_cast<cudaStream_t>(stream));
+    return launch_any(p, args_of(p, false), false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, void* stream) {
@@ -768,7 +789,7 @@ extern "C" int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, vo
     }
     if (p->length && (!p->x || !p->forget || !p->dy || !p->states || !p->dx || !p->dforget || (p->z && !p->dz)))
         return fail(SSM_ERR_INVALID, "gated_linear_recurrence bwd: null pointer");
-    Args a = args_of(p);
+    Args a = args_of(p, true);
     if (p->dlower) {
         size_t need = 0;
         ssm_gated_recurrence_sizes(p, nullptr, &need);
@@ -778,7 +799,7 @@ extern "C" int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, vo
     }
     if (int s = launch_any(p, a, true, st)) return s;
     if (p->dlower) {
-        fold_kernel<<<(unsigned)ceil_div(a.dim, 256), 256, 0, st>>>(a.part, a.batch * cluster_of(p), a.dim, p->dlower);
+        fold_kernel<<<(unsigned)ceil_div(a.dim, 256), 256, 0, st>>>(a.part, a.batch * cluster_of(p, true), a.dim, p->dlower);
         return check_launch("gated_linear_recurrence bwd: fold");
     }
     return SSM_OK;
