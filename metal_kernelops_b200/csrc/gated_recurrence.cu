@@ -24,8 +24,7 @@
 // time from the right start.  A CTA's kWarps warps make a chunk.  Where the channel
 // tiles of all batch rows do not fill the GPU, a cluster of CTAs takes consecutive
 // chunks of one tile at a time, and its CTAs exchange their chunks' maps through
-// distributed shared memory, one cluster barrier for each such round; the inputs
-// are still read once.  Chunks come through a ring of shared-memory stages that TMA
+// distributed shared memory; the inputs are still read once.  Chunks come through a ring of shared-memory stages that TMA
 // fills ahead (rows that do not start on 16-byte boundaries are read directly).
 // A composition whose A is exactly 0 (a reset) takes H alone: a state that is not
 // finite does not pass a reset.
@@ -249,8 +248,56 @@ __device__ __forceinline__ Map<F> then(const Map<F>& first, const Map<F>& next) 
     return {mu(first.A, next.A), through<RESET>(next.A, next.H, first.H)};
 }
 
-// A cluster of C CTAs takes C consecutive chunks at a time: its CTAs exchange
-// their chunks' maps through each other's shared memory, once a round.
+// A cluster of C CTAs takes C consecutive chunks at a time (a round): each CTA
+// sends its chunk's map to all of them with asynchronous remote stores that
+// count their bytes on the receiver's mbarrier, and waits for the C maps of the
+// round.  No fence is involved: a cluster barrier's release would first wait for
+// the round's global stores (a round of 4 x 64 steps took 4 us with one).
+// Two buffers alternate: a CTA sends round n + 2 only after it has every map of
+// round n + 1, which a peer sends after all its warps have read round n.
+__device__ __forceinline__ uint32_t remote(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void send(uint32_t addr, uint32_t bar, float a, float h) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+                 :: "r"(addr), "r"(__float_as_uint(a)), "r"(__float_as_uint(h)), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void send(uint32_t addr, uint32_t bar, float2 a, float2 h) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                 :: "r"(addr), "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(h.x)),
+                    "r"(__float_as_uint(h.y)), "r"(bar) : "memory");
+}
+template <typename F>
+struct alignas(128) Exchange {        // whole 128-byte lines: the ring behind it starts on one
+    Map<F> far[2][kMaxCluster][32];
+    uint64_t bars[2];
+    __device__ __forceinline__ void arm(int s, int C) {
+        tc::mbar_expect_tx(tc::smem_u32(&bars[s]), (uint32_t)(C * 32 * sizeof(Map<F>)));
+    }
+    __device__ __forceinline__ void init(int C) {
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < 2; ++s) tc::mbar_init(tc::smem_u32(&bars[s]), 1);
+            tc::fence_mbar_init();
+            arm(0, C);
+            arm(1, C);
+        }
+    }
+    // One warp: its lanes' maps of the whole chunk to every CTA.
+    __device__ __forceinline__ void put(int64_t round, int rank, int C, const Map<F>& all) {
+        const int s = (int)(round & 1);
+        const uint32_t at = tc::smem_u32(&far[s][rank][threadIdx.x & 31]), bar = tc::smem_u32(&bars[s]);
+        for (int r = 0; r < C; ++r) send(remote(at, r), remote(bar, r), all.A, all.H);
+    }
+    // Every thread: the round's maps are here.
+    __device__ __forceinline__ bool wait(int64_t round, int C) {
+        const int s = (int)(round & 1);
+        const bool ok = tc::mbar_wait(tc::smem_u32(&bars[s]), (uint32_t)(round >> 1) & 1u);
+        if (threadIdx.x == 0) arm(s, C);
+        return ok;
+    }
+};
 __device__ __forceinline__ int cluster_size() { return (int)cooperative_groups::this_cluster().num_blocks(); }
 
 template <typename T, bool GATE, bool RESET, bool TMA, int ST, int N>
@@ -260,7 +307,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     constexpr int E = Lane<T>::E, NT = GATE ? 3 : 2, kChunk = kWarps * N;
     const Args& a = ta.a;
     __shared__ Map<F> maps[2][kWarps][32];
-    __shared__ Map<F> far[2][kMaxCluster][32];
+    __shared__ Exchange<F> ex;
     extern __shared__ __align__(128) uint8_t smem[];
     const Ring<NT, ST, N> ring{smem};
     const int which[3] = {0, 1, 2};
@@ -269,7 +316,10 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.y, tile = blockIdx.x / C, c = (tile * 32 + lane) * E;
     const int64_t rounds = (a.chunks + C - 1) / C;
-    if (C > 1) cluster.sync();                          // every CTA's shared memory is there to write to
+    if (C > 1) {
+        ex.init(C);
+        cluster.sync();                                 // every CTA's barriers are there to write to
+    }
     if constexpr (TMA) {
         ring.init();
         if (threadIdx.x == 0)
@@ -335,16 +385,19 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
             }
         } else {
             Map<F> before{same<F>(1.0f), same<F>(0.0f)};
-            for (int w = 0; w < warp; ++w) before = then<RESET>(before, mw[w][lane]);
-            if (warp == kWarps - 1) {
-                const Map<F> all = then<RESET>(before, m);
-                for (int r = 0; r < C; ++r) cluster.map_shared_rank(&far[n & 1][0][0], r)[rank * 32 + lane] = all;
-            }
-            cluster.sync();
-            for (int r = 0; r < C; ++r) {
-                if (r == rank) h = S;
-                const Map<F> o = far[n & 1][r][lane];
-                S = through<RESET>(o.A, o.H, S);
+#pragma unroll
+            for (int w = 0; w < kWarps - 1; ++w)
+                if (w < warp) before = then<RESET>(before, mw[w][lane]);
+            if (warp == kWarps - 1) ex.put(n, rank, C, then<RESET>(before, m));
+            if (!ex.wait(n, C) && lane == 0) report(a, 113);
+            h = S;
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+                if (r < C) {
+                    if (r == rank) h = S;
+                    const Map<F> o = ex.far[n & 1][r][lane];
+                    S = through<RESET>(o.A, o.H, S);
+                }
             }
             h = through<RESET>(before.A, before.H, h);
         }
@@ -366,6 +419,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
             else if (i < live) st_word<T>(y + i * a.dim, o, c, a.dim, a.words);
         }
     }
+    if (C > 1) cluster.sync();                          // nothing is on its way to a CTA that ends
     if (warp == 0 && rank == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
 }
 
@@ -376,7 +430,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
     constexpr int E = Lane<T>::E, NT = GATE ? 4 : 3, kChunk = kWarps * N;
     const Args& a = ta.a;
     __shared__ struct { Map<F> m[32]; F R[32]; } maps[2][kWarps];
-    __shared__ Map<F> far[2][kMaxCluster][32];          // H holds R here
+    __shared__ Exchange<F> ex;            // of (A, R)
     __shared__ F sums[kWarps][32];
     extern __shared__ __align__(128) uint8_t smem[];
     const Ring<NT, ST, N> ring{smem};
@@ -386,7 +440,10 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.y, tile = blockIdx.x / C, c = (tile * 32 + lane) * E;
     const int64_t rounds = (a.chunks + C - 1) / C;
-    if (C > 1) cluster.sync();                          // every CTA's shared memory is there to write to
+    if (C > 1) {
+        ex.init(C);
+        cluster.sync();                                 // every CTA's barriers are there to write to
+    }
     if constexpr (TMA) {
         ring.init();
         if (threadIdx.x == 0)
@@ -465,22 +522,28 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
             }
         } else {
             Map<F> after{one, zero};
-            for (int w = kWarps - 1; w > warp; --w) after = then<RESET>(after, Map<F>{mw[w].m[lane].A, mw[w].R[lane]});
-            if (warp == 0) {
-                const Map<F> all = then<RESET>(after, Map<F>{m.A, d});
-                for (int r = 0; r < C; ++r) cluster.map_shared_rank(&far[turn & 1][0][0], r)[rank * 32 + lane] = all;
-            }
-            cluster.sync();
-            for (int r = C - 1; r >= 0; --r) {
-                if (r == rank) d = D;
-                const Map<F> o = far[turn & 1][r][lane];
-                D = through<RESET>(o.A, o.H, D);
+#pragma unroll
+            for (int w = kWarps - 1; w > 0; --w)
+                if (w > warp) after = then<RESET>(after, Map<F>{mw[w].m[lane].A, mw[w].R[lane]});
+            if (warp == 0) ex.put(turn, rank, C, then<RESET>(after, Map<F>{m.A, d}));
+            if (!ex.wait(turn, C) && lane == 0) report(a, 114);
+            d = D;
+#pragma unroll
+            for (int r = kMaxCluster - 1; r >= 0; --r) {
+                if (r < C) {
+                    if (r == rank) d = D;
+                    const Map<F> o = ex.far[turn & 1][r][lane];
+                    D = through<RESET>(o.A, o.H, D);
+                }
             }
             d = through<RESET>(after.A, after.H, d);
         }
-        for (int w = 0; w < warp; ++w) {
-            const Map<F> o = mw[w].m[lane];
-            h = through<RESET>(o.A, o.H, h);
+#pragma unroll
+        for (int w = 0; w < kWarps - 1; ++w) {
+            if (w < warp) {
+                const Map<F> o = mw[w].m[lane];
+                h = through<RESET>(o.A, o.H, h);
+            }
         }
         again(xw);
         again(k);
@@ -524,6 +587,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         }
         dlower = sub(dlower, dl);
     }
+    if (C > 1) cluster.sync();                          // nothing is on its way to a CTA that ends
     if (warp == 0 && rank == 0 && a.dinit != nullptr) st_chan(a.dinit + b * a.dim, c, a.dim, D);
     if (a.part != nullptr) {
         sums[warp][lane] = dlower;
