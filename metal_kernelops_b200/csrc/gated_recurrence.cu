@@ -24,8 +24,10 @@
 // time from the right start.  A CTA's kWarps warps make a chunk.  Where the channel
 // tiles of all batch rows do not fill the GPU, a cluster of CTAs takes consecutive
 // chunks of one tile at a time, and its CTAs exchange their chunks' maps through
-// distributed shared memory; the inputs are still read once.  Chunks come through a ring of shared-memory stages that TMA
-// fills ahead (rows that do not start on 16-byte boundaries are read directly).
+// distributed shared memory; the inputs are still read once.  Chunks come through a
+// ring of shared-memory stages filled ahead: by TMA, by 4-byte asynchronous copies
+// where rows do not start on 16-byte boundaries; odd widths of 16-bit data are
+// read directly.
 // A composition whose A is exactly 0 (a reset) takes H alone: a state that is not
 // finite does not pass a reset.
 // The forward saves the state that enters each chunk, in fp32, for the backward,
@@ -66,6 +68,7 @@ struct Args {
 struct TmaArgs {
     Args a;
     alignas(64) CUtensorMap m[4];
+    int cluster;                                    // host: the launch's cluster size
 };
 
 __device__ int g_glr_error;
@@ -192,9 +195,10 @@ __device__ __forceinline__ void ld_steps(const void* base, int64_t row, int64_t 
     for (int i = 0; i < N; ++i) w[i] = i < live ? ld_word<T>(p + i * stride, c, a.dim, a.words) : 0u;
 }
 
-// The ring of chunk tiles in shared memory that TMA fills: stage s holds NT
-// tensors' chunks, a warp's steps being N consecutive 128-byte rows of each.
-// Thread 0 issues; the wait of a stage is every thread's.
+// The ring of chunk tiles in shared memory: stage s holds NT tensors' chunks, a warp's steps being N consecutive 128-byte rows of each.
+// TMA: thread 0 issues, the wait of a stage is every thread's.  kWords: each lane
+// copies the words that it will read itself, so its own wait is enough.
+enum Loads { kDirect, kWords, kTma };
 template <int NT, int ST, int N>
 struct Ring {
     static constexpr int kTile = kWarps * N * kRow;   // bytes of one tensor's chunk
@@ -215,6 +219,18 @@ struct Ring {
         tc::mbar_expect_tx(bar(s), NT * kTile);
         for (int i = 0; i < NT; ++i)
             tc::tma_load3(tc::smem_u32(base + (s * NT + i) * kTile), &ta.m[which[i]], c0, (int)t, b, bar(s));
+    }
+    // The lane's words of tensor i: N steps from p, `live` of them inside the sequence.
+    template <typename T>
+    __device__ __forceinline__ void copy(int s, int i, const void* tensor, int64_t row, int64_t stride, int64_t t,
+                                         int live, int64_t c, int64_t dim) const {
+        const T* p = static_cast<const T*>(tensor) + row + t * stride + c;
+        const uint32_t d = tc::smem_u32(base + (s * NT + i) * kTile) + (threadIdx.x / 32 * N * 32 + (threadIdx.x & 31)) * 4;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const bool in = k < live && c < dim;
+            tc::cp_async4_zfill(d + k * kRow, in ? static_cast<const void*>(p + k * stride) : tensor, in ? 4u : 0u);
+        }
     }
     __device__ __forceinline__ void read(int s, int i, uint32_t* w) const {
         const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (s * NT + i) * kTile) + threadIdx.x / 32 * N * 32 +
@@ -300,7 +316,7 @@ struct alignas(128) Exchange {        // whole 128-byte lines: the ring behind i
 };
 __device__ __forceinline__ int cluster_size() { return (int)cooperative_groups::this_cluster().num_blocks(); }
 
-template <typename T, bool GATE, bool RESET, bool TMA, int ST, int N>
+template <typename T, bool GATE, bool RESET, int LOADS, int ST, int N>
 __global__ void __launch_bounds__(kThreads, N > 8 ? 2 : 3)
 fwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
@@ -320,11 +336,24 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
         ex.init(C);
         cluster.sync();                                 // every CTA's barriers are there to write to
     }
-    if constexpr (TMA) {
-        ring.init();
-        if (threadIdx.x == 0)
-            for (int s = 0; s < ST && s < rounds; ++s)
-                ring.load(ta, s, (int)(tile * 32 * E), ((int64_t)s * C + rank) * kChunk, (int)b, which);
+    // the chunk of round n into its stage
+    auto fill = [&](int64_t n) {
+        const int s = (int)(n % ST);
+        const int64_t t0 = (n * C + rank) * kChunk;
+        if constexpr (LOADS == kTma) {
+            if (threadIdx.x == 0) ring.load(ta, s, (int)(tile * 32 * E), t0, (int)b, which);
+        } else if constexpr (LOADS == kWords) {
+            const int64_t t = t0 + warp * N;
+            const int live = (int)max64(0, min64(N, a.length - t));
+            ring.template copy<T>(s, 0, a.x, b * a.xb, a.xt, t, live, c, a.dim);
+            ring.template copy<T>(s, 1, a.forget, b * a.fb, a.ft, t, live, c, a.dim);
+            if (GATE) ring.template copy<T>(s, 2, a.z, b * a.zb, a.zt, t, live, c, a.dim);
+        }
+    };
+    if constexpr (LOADS == kTma) ring.init();
+    for (int s = 0; s < ST; ++s) {
+        if (s < rounds) fill(s);
+        if constexpr (LOADS == kWords) tc::cp_async_commit();
     }
     F span, nspan, S;
     ld_chan(a.lower, c, a.dim, 0.0f, span);
@@ -339,9 +368,13 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
         const uint32_t rs = RESET ? reset_mask<N>(a.reset, b * a.length, t, a.length) : 0u;
         {
             uint32_t xw[N], fw[N];
-            if constexpr (TMA) {
+            if constexpr (LOADS != kDirect) {
                 const int s = (int)(n % ST);
-                if (!tc::mbar_wait(ring.bar(s), (uint32_t)(n / ST) & 1u) && lane == 0) report(a, 111);
+                if constexpr (LOADS == kTma) {
+                    if (!tc::mbar_wait(ring.bar(s), (uint32_t)(n / ST) & 1u) && lane == 0) report(a, 111);
+                } else {
+                    tc::cp_async_wait<ST - 1>();
+                }
                 ring.read(s, 0, xw);
                 ring.read(s, 1, fw);
                 if (GATE) ring.read(s, 2, zw);
@@ -372,8 +405,8 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
         mw[warp][lane] = m;
         __syncthreads();
         // every warp has its words in registers: the stage is free
-        if (TMA && threadIdx.x == 0 && n + ST < rounds)
-            ring.load(ta, (int)(n % ST), (int)(tile * 32 * E), ((n + ST) * C + rank) * kChunk, (int)b, which);
+        if (n + ST < rounds) fill(n + ST);
+        if constexpr (LOADS == kWords) tc::cp_async_commit();          // one group a round
         F h;
         if (C == 1) {
             h = S;
@@ -423,7 +456,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     if (warp == 0 && rank == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
 }
 
-template <typename T, bool GATE, bool RESET, bool TMA, int ST, int N>
+template <typename T, bool GATE, bool RESET, int LOADS, int ST, int N>
 __global__ void __launch_bounds__(kThreads, 2)
 bwd_kernel(const __grid_constant__ TmaArgs ta) {
     using F = typename Lane<T>::F;
@@ -444,11 +477,25 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         ex.init(C);
         cluster.sync();                                 // every CTA's barriers are there to write to
     }
-    if constexpr (TMA) {
-        ring.init();
-        if (threadIdx.x == 0)
-            for (int s = 0; s < ST && s < rounds; ++s)
-                ring.load(ta, s, (int)(tile * 32 * E), ((rounds - 1 - s) * C + rank) * kChunk, (int)b, which);
+    // the chunk of a turn into its stage
+    auto fill = [&](int64_t turn) {
+        const int s = (int)(turn % ST);
+        const int64_t t0 = ((rounds - 1 - turn) * C + rank) * kChunk;
+        if constexpr (LOADS == kTma) {
+            if (threadIdx.x == 0) ring.load(ta, s, (int)(tile * 32 * E), t0, (int)b, which);
+        } else if constexpr (LOADS == kWords) {
+            const int64_t t = t0 + warp * N;
+            const int live = (int)max64(0, min64(N, a.length - t));
+            ring.template copy<T>(s, 0, a.x, b * a.xb, a.xt, t, live, c, a.dim);
+            ring.template copy<T>(s, 1, a.forget, b * a.fb, a.ft, t, live, c, a.dim);
+            ring.template copy<T>(s, 2, a.dy, b * a.dyb, a.dyt, t, live, c, a.dim);
+            if (GATE) ring.template copy<T>(s, 3, a.z, b * a.zb, a.zt, t, live, c, a.dim);
+        }
+    };
+    if constexpr (LOADS == kTma) ring.init();
+    for (int s = 0; s < ST; ++s) {
+        if (s < rounds) fill(s);
+        if constexpr (LOADS == kWords) tc::cp_async_commit();
     }
     const F one = same<F>(1.0f), zero = same<F>(0.0f);
     F span, nspan, D;
@@ -466,9 +513,13 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         ld_chan(chunk < a.chunks ? a.states + (b * a.saved + chunk) * a.dim : nullptr, c, a.dim, 0.0f, h);
         {
             uint32_t fw[N];
-            if constexpr (TMA) {
+            if constexpr (LOADS != kDirect) {
                 const int s = (int)(turn % ST);
-                if (!tc::mbar_wait(ring.bar(s), (uint32_t)(turn / ST) & 1u) && lane == 0) report(a, 112);
+                if constexpr (LOADS == kTma) {
+                    if (!tc::mbar_wait(ring.bar(s), (uint32_t)(turn / ST) & 1u) && lane == 0) report(a, 112);
+                } else {
+                    tc::cp_async_wait<ST - 1>();
+                }
                 ring.read(s, 0, xw);
                 ring.read(s, 1, fw);
                 ring.read(s, 2, dw);
@@ -509,9 +560,8 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         mw[warp].m[lane] = m;
         mw[warp].R[lane] = d;
         __syncthreads();
-        if (TMA && threadIdx.x == 0 && turn + ST < rounds)
-            ring.load(ta, (int)(turn % ST), (int)(tile * 32 * E), ((rounds - 1 - turn - ST) * C + rank) * kChunk, (int)b,
-                      which);
+        if (turn + ST < rounds) fill(turn + ST);
+        if constexpr (LOADS == kWords) tc::cp_async_commit();          // one group a turn
         if (C == 1) {
             d = D;
 #pragma unroll
@@ -728,21 +778,53 @@ static bool tma_ok(const Args& a, int dtype, bool bwd) {
            (!bwd || ok(a.dy, a.dyt, a.dyb));
 }
 
-// CTAs of a cluster: as many (a power of two, up to 8, no more than chunks) as
-// bring the grid to two CTAs per SM.
-static int cluster_of(const ssm_gated_recurrence_params* p, bool bwd) {
-    const int64_t tiles = ceil_div(p->dim * esize(p->dtype), kRow);
-    const int64_t chunks = ceil_div(p->length, kWarps * (bwd ? kBwdSteps : kFwdSteps));
-    int c = 1;
-    while (c < kMaxCluster && 2 * c <= chunks && tiles * p->batch * c < 148 * 2) c *= 2;
-    return c;
+// CTAs of a cluster.  With C of them a tile takes ceil(chunks / C) rounds, and the
+// tiles run in as many waves as the GPU's room for such clusters needs; a round of a
+// cluster costs 12 % and 6 % more per CTA than a lone CTA's (the exchange, and the
+// spread of its CTAs).  The C with the least product is taken.  Measured at 1 x 4096
+// x 5120 bf16 with gate (80 tiles, room for 296 CTAs): forward 83 us with C = 1, 67
+// with 2, 52 with 3, 60 with 4; at 2 x 16384 x 5120 (160 tiles): 437 with 1, 386
+// with 2, 308 with 5; at 16 x 4096 x 5120 (1280 tiles) C = 1 is best.
+template <auto kernel>
+static int cluster_of(int64_t tiles, int64_t chunks, size_t smem) {
+    static int room[kMaxCluster + 1];              // clusters that fit at once, by size; 0: not asked yet
+    double best = 0.0;
+    int size = 1;
+    for (int c = 1; c <= kMaxCluster && c <= chunks; ++c) {
+        if (room[c] == 0) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(c);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = c;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+                cudaGetLastError();
+                n = 148 * 2 / c;
+            }
+            room[c] = n;
+        }
+        const double cost = (double)ceil_div(tiles, room[c]) * (double)ceil_div(chunks, c) *
+                            (c == 1 ? 1.0 : 1.0 + 0.06 * c);
+        if (c == 1 || cost < best) {
+            best = cost;
+            size = c;
+        }
+    }
+    return size;
 }
 
-template <typename K>
-static int launch_kernel(K kernel, const TmaArgs& ta, unsigned tiles, int cluster, size_t smem, cudaStream_t st,
-                         const char* what) {
+template <auto kernel>
+static int launch_kernel(TmaArgs& ta, unsigned tiles, size_t smem, cudaStream_t st, const char* what) {
     if (smem && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return check_launch(what);
+    const int cluster = cluster_of<kernel>((int64_t)tiles * ta.a.batch, ta.a.chunks, smem);
+    ta.cluster = cluster;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(tiles * cluster, (unsigned)ta.a.batch);
     cfg.blockDim = dim3(kThreads);
@@ -760,32 +842,39 @@ static int launch_kernel(K kernel, const TmaArgs& ta, unsigned tiles, int cluste
 
 constexpr int kFwdStages = 2, kBwdStages = 2;
 
-template <typename T, bool GATE, bool RESET>
-static int launch(const TmaArgs& ta, bool bwd, bool tma, int cluster, cudaStream_t st) {
+template <typename T, bool GATE, bool RESET, int LOADS>
+static int launch(TmaArgs& ta, bool bwd, cudaStream_t st) {
     const unsigned tiles = (unsigned)ceil_div(ta.a.dim, 32 * Lane<T>::E);
-    constexpr size_t fs = Ring<GATE ? 3 : 2, kFwdStages, kFwdSteps>::bytes,
-                     bs = Ring<GATE ? 4 : 3, kBwdStages, kBwdSteps>::bytes;
-    if (bwd) {
-        const char* what = "gated_linear_recurrence bwd";
-        if (tma) return launch_kernel(bwd_kernel<T, GATE, RESET, true, kBwdStages, kBwdSteps>, ta, tiles, cluster, bs, st, what);
-        return launch_kernel(bwd_kernel<T, GATE, RESET, false, kBwdStages, kBwdSteps>, ta, tiles, cluster, 0, st, what);
-    }
-    const char* what = "gated_linear_recurrence fwd";
-    if (tma) return launch_kernel(fwd_kernel<T, GATE, RESET, true, kFwdStages, kFwdSteps>, ta, tiles, cluster, fs, st, what);
-    return launch_kernel(fwd_kernel<T, GATE, RESET, false, kFwdStages, kFwdSteps>, ta, tiles, cluster, 0, st, what);
+    constexpr size_t fs = LOADS == kDirect ? 0 : Ring<GATE ? 3 : 2, kFwdStages, kFwdSteps>::bytes;
+    constexpr size_t bs = LOADS == kDirect ? 0 : Ring<GATE ? 4 : 3, kBwdStages, kBwdSteps>::bytes;
+    if (bwd)
+        return launch_kernel<bwd_kernel<T, GATE, RESET, LOADS, kBwdStages, kBwdSteps>>(
+            ta, tiles, bs, st, "gated_linear_recurrence bwd");
+    return launch_kernel<fwd_kernel<T, GATE, RESET, LOADS, kFwdStages, kFwdSteps>>(
+        ta, tiles, fs, st, "gated_linear_recurrence fwd");
+}
+
+template <typename T, bool GATE, bool RESET>
+static int launch_loads(TmaArgs& ta, bool bwd, int loads, cudaStream_t st) {
+    if (loads == kTma) return launch<T, GATE, RESET, kTma>(ta, bwd, st);
+    if (loads == kWords || sizeof(T) == 4) return launch<T, GATE, RESET, kWords>(ta, bwd, st);
+    if constexpr (sizeof(T) == 2) return launch<T, GATE, RESET, kDirect>(ta, bwd, st);
+    return SSM_OK;
 }
 
 template <typename T>
-static int launch_gate(const TmaArgs& ta, bool bwd, bool tma, int cluster, cudaStream_t st) {
+static int launch_gate(TmaArgs& ta, bool bwd, int loads, cudaStream_t st) {
     if (ta.a.reset)
-        return ta.a.z ? launch<T, true, true>(ta, bwd, tma, cluster, st) : launch<T, false, true>(ta, bwd, tma, cluster, st);
-    return ta.a.z ? launch<T, true, false>(ta, bwd, tma, cluster, st) : launch<T, false, false>(ta, bwd, tma, cluster, st);
+        return ta.a.z ? launch_loads<T, true, true>(ta, bwd, loads, st) : launch_loads<T, false, true>(ta, bwd, loads, st);
+    return ta.a.z ? launch_loads<T, true, false>(ta, bwd, loads, st) : launch_loads<T, false, false>(ta, bwd, loads, st);
 }
 
-static int launch_any(const ssm_gated_recurrence_params* p, const Args& a, bool bwd, cudaStream_t st) {
+static int launch_any(const ssm_gated_recurrence_params* p, const Args& a, bool bwd, cudaStream_t st,
+                      int* cluster = nullptr) {
     TmaArgs ta{};
     ta.a = a;
     const bool tma = tma_ok(a, p->dtype, bwd);
+    const int loads = tma ? kTma : a.words ? kWords : kDirect;
     const int chunk = kWarps * (bwd ? kBwdSteps : kFwdSteps);
     if (tma) {
         if (int s = ensure_context("gated_linear_recurrence")) return s;
@@ -796,10 +885,11 @@ static int launch_any(const ssm_gated_recurrence_params* p, const Args& a, bool 
         if (bwd)
             if (int s = encode(&ta.m[3], a.dy, a.dyt, a.dyb, p->dtype, chunk, a)) return s;
     }
-    const int cluster = cluster_of(p, bwd);
-    if (p->dtype == SSM_F32) return launch_gate<float>(ta, bwd, tma, cluster, st);
-    if (p->dtype == SSM_BF16) return launch_gate<__nv_bfloat16>(ta, bwd, tma, cluster, st);
-    return launch_gate<__half>(ta, bwd, tma, cluster, st);
+    const int s = p->dtype == SSM_F32 ? launch_gate<float>(ta, bwd, loads, st)
+                  : p->dtype == SSM_BF16 ? launch_gate<__nv_bfloat16>(ta, bwd, loads, st)
+                                         : launch_gate<__half>(ta, bwd, loads, st);
+    if (cluster) *cluster = ta.cluster;
+    return s;
 }
 
 template <typename T>
@@ -831,7 +921,7 @@ extern "C" int ssm_gated_recurrence_sizes(const ssm_gated_recurrence_params* p, 
                                           size_t* workspace_bytes) {
     if (int s = validate(p)) return s;
     if (states_bytes) *states_bytes = (size_t)(p->batch * ceil_div(p->length, kWarps * kBwdSteps) * p->dim) * 4;
-    if (workspace_bytes) *workspace_bytes = (size_t)(p->batch * cluster_of(p, true) * p->dim) * 4;
+    if (workspace_bytes) *workspace_bytes = (size_t)(p->batch * kMaxCluster * p->dim) * 4;
     return SSM_OK;
 }
 
@@ -861,9 +951,10 @@ extern "C" int ssm_gated_recurrence_bwd(const ssm_gated_recurrence_params* p, vo
             return fail(SSM_ERR_WORKSPACE, "gated_linear_recurrence bwd: workspace smaller than ssm_gated_recurrence_sizes");
         a.part = static_cast<float*>(p->workspace);
     }
-    if (int s = launch_any(p, a, true, st)) return s;
+    int cluster = 1;
+    if (int s = launch_any(p, a, true, st, &cluster)) return s;
     if (p->dlower) {
-        fold_kernel<<<(unsigned)ceil_div(a.dim, 256), 256, 0, st>>>(a.part, a.batch * cluster_of(p, true), a.dim, p->dlower);
+        fold_kernel<<<(unsigned)ceil_div(a.dim, 256), 256, 0, st>>>(a.part, a.batch * cluster, a.dim, p->dlower);
         return check_launch("gated_linear_recurrence bwd: fold");
     }
     return SSM_OK;

@@ -210,6 +210,10 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t saddr, const void* g, 
 __device__ __forceinline__ void cp_async8(uint32_t saddr, const void* g) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(saddr), "l"(g) : "memory");
 }
+// 4-byte copy, or 4 zero bytes for src_bytes = 0.
+__device__ __forceinline__ void cp_async4_zfill(uint32_t saddr, const void* g, uint32_t src_bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(saddr), "l"(g), "r"(src_bytes) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
