@@ -533,6 +533,43 @@ int ssm_add_rmsnorm_bwd(const ssm_add_rmsnorm_params* p, void* stream);
 int ssm_quantize_int8(const ssm_add_rmsnorm_params* p, void* stream);
 
 /* ------------------------------------------------------------------------- *
+ * Linear layer in 8-bit integers, with a scale per token and per output
+ * feature.  No counterpart in the reference.
+ *
+ *     out[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] (+ bias[n])
+ *
+ *   x (tokens, in_features), w (out_features, in_features): int8
+ *   x_scale (tokens), w_scale (out_features), bias (out_features): fp32
+ *                                                  (bias NULL: none)
+ *   out (tokens, out_features): out_dtype, dense
+ * The sum is exact (int32); in_features is at most 131071.  Rows whose base or
+ * stride is not a multiple of 16 bytes are copied to the workspace first
+ * (ssm_int8_linear_sizes, zero for aligned rows; query with the pointers set).
+ * ------------------------------------------------------------------------- */
+typedef struct ssm_int8_linear_params {
+    int64_t tokens, in_features, out_features;
+    int64_t x_row_stride, w_row_stride;   /* elements between rows (0: in_features) */
+    int32_t out_dtype;
+    uint32_t flags;             /* none defined */
+    const int8_t* x;
+    const float* x_scale;
+    const int8_t* w;
+    const float* w_scale;
+    const float* bias;
+    void* out;
+    void* workspace;
+    size_t workspace_bytes;
+    /* optional device word (NULL: none).  A kernel of this op that gives up
+     * on a bounded wait writes its non-zero code here (the first failure
+     * wins; the word is never cleared by the library), besides the per-device
+     * flag that ssm_take_kernel_error reads.  Start it at 0. */
+    int32_t* status;
+} ssm_int8_linear_params;
+
+int ssm_int8_linear_sizes(const ssm_int8_linear_params* p, size_t* workspace_bytes);
+int ssm_int8_linear_fwd(const ssm_int8_linear_params* p, void* stream);
+
+/* ------------------------------------------------------------------------- *
  * Gated linear recurrence: one state per channel, a forget gate per token.  No
  * counterpart in the reference.
  *

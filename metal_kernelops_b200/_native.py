@@ -49,7 +49,7 @@ EXPORTS = (
     "ssm_gated_rmsnorm_sizes", "ssm_gated_rmsnorm_fwd", "ssm_gated_rmsnorm_bwd",
     "ssm_add_rmsnorm_sizes", "ssm_add_rmsnorm_fwd", "ssm_add_rmsnorm_bwd", "ssm_quantize_int8",
     "ssm_gated_recurrence_sizes", "ssm_gated_recurrence_fwd", "ssm_gated_recurrence_bwd",
-    "ssm_gated_recurrence_step",
+    "ssm_gated_recurrence_step", "ssm_int8_linear_sizes", "ssm_int8_linear_fwd",
 )
 
 _I64, _I32, _U32, _P, _SZ = ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_size_t
@@ -163,6 +163,17 @@ class AddRmsNormParams(ctypes.Structure):
     ]
 
 
+class Int8LinearParams(ctypes.Structure):
+    _fields_ = [
+        ("tokens", _I64), ("in_features", _I64), ("out_features", _I64),
+        ("x_row_stride", _I64), ("w_row_stride", _I64),
+        ("out_dtype", _I32), ("flags", _U32),
+        ("x", _P), ("x_scale", _P), ("w", _P), ("w_scale", _P), ("bias", _P), ("out", _P),
+        ("workspace", _P), ("workspace_bytes", _SZ),
+        ("status", _P),
+    ]
+
+
 class GatedRecurrenceParams(ctypes.Structure):
     _fields_ = [
         ("batch", _I64), ("length", _I64), ("dim", _I64),
@@ -233,6 +244,9 @@ def lib():
             handle.ssm_add_rmsnorm_sizes.argtypes = [ctypes.POINTER(AddRmsNormParams), ctypes.POINTER(_SZ)]
             handle.ssm_gated_recurrence_sizes.argtypes = [
                 ctypes.POINTER(GatedRecurrenceParams), ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]
+            handle.ssm_int8_linear_fwd.restype = ctypes.c_int
+            handle.ssm_int8_linear_fwd.argtypes = [ctypes.POINTER(Int8LinearParams), ctypes.c_void_p]
+            handle.ssm_int8_linear_sizes.argtypes = [ctypes.POINTER(Int8LinearParams), ctypes.POINTER(_SZ)]
             handle.ssm_gated_recurrence_step.restype = ctypes.c_int
             handle.ssm_gated_recurrence_step.argtypes = [ctypes.POINTER(GatedRecurrenceStepParams),
                                                          ctypes.c_void_p]
@@ -251,7 +265,7 @@ def lib():
             for name in ("ssm_selective_scan_sizes", "ssm_state_update_sizes", "ssm_chunk_scan_sizes",
                          "ssm_ss2d_scan_sizes", "ssm_selective_scan_fwd_workspace",
                          "ssm_causal_conv1d_sizes", "ssm_gated_rmsnorm_sizes", "ssm_add_rmsnorm_sizes",
-                         "ssm_gated_recurrence_sizes"):
+                         "ssm_gated_recurrence_sizes", "ssm_int8_linear_sizes"):
                 getattr(handle, name).restype = ctypes.c_int
             handle.ssm_take_kernel_error.restype = ctypes.c_int
             handle.ssm_take_kernel_error.argtypes = []

@@ -1,0 +1,365 @@
+// Linear layer in 8-bit integers for sm_100a:
+//     out[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] (+ bias[n])
+// x (tokens, K) and w (features, K) int8 rows, the sum exact in int32 (K is at
+// most 131071, so that 128 * 128 * K stays below 2^31), the two scales and the
+// bias applied in fp32, one rounding to the output's type.
+//
+// The products run on the fifth-generation tensor cores (kind::i8), operands staged
+// by TMA in the 128-byte swizzle, int32 accumulators in tensor memory.  Rows past the
+// end and the last bytes of K arrive as zeros.  TMA wants rows on 16-byte
+// boundaries: operands that are not are first copied to such rows in the workspace.
+//
+// Few tokens: reading w once is the whole cost.  `skinny_kernel` makes the features
+// the 128 rows of the product and the tokens its columns (16 to 128), and cuts K
+// over the CTAs of a cluster until the GPU is full; the slices' int32 sums are added
+// through distributed shared memory, exactly, so the cut changes no result.
+#include <cooperative_groups.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <climits>
+#include <mutex>
+
+#include "common.cuh"
+#include "tc.cuh"
+
+namespace ssm {
+namespace i8 {
+
+constexpr int kBlockK = 128;                        // bytes of K a stage holds: one swizzle row
+constexpr int kFeatures = 128;                      // features of a skinny tile
+constexpr int kMaxStages = 8;
+
+struct Args {
+    int64_t tokens, features, k;
+    const float* xs; const float* ws; const float* bias;
+    void* out;
+    int out_dtype;
+    int vec;                                        // 16-byte stores are aligned
+    int* status;
+};
+struct TmaArgs {
+    Args a;
+    alignas(64) CUtensorMap mx, mw;
+    int stages;
+};
+
+__device__ int g_i8_error;
+
+__device__ __forceinline__ void report(const Args& a, int code) {
+    atomicCAS(&g_i8_error, 0, code);
+    if (a.status) atomicCAS(a.status, 0, code);
+}
+
+// Shared-memory descriptor of K-major rows of 128 bytes in the 128-byte swizzle:
+// eight rows make an atom of 1024 bytes, the next eight follow.
+__device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+// Instruction descriptor of kind::i8: signed 8-bit A and B, both K-major, int32 D.
+__host__ __device__ constexpr uint32_t idesc_i8(uint32_t M, uint32_t N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+        :: "r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+// 32 lanes x 16 columns of int32; wait_ld orders the registers' uses after the wait.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void wait_ld16(int* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
+
+// ------------------------------------------------------------ few tokens --
+template <int NT>
+struct Skinny {
+    static constexpr int kStage = kFeatures * kBlockK + NT * kBlockK;     // bytes: w rows, then x rows
+    static constexpr uint32_t kTmem = NT < 32 ? 32 : NT;
+    static size_t smem(int stages) { return (size_t)stages * kStage + 1024; }
+    // the K slices' sums meet in the stages' memory
+    static int min_stages() { return (NT * kFeatures * 4 + kStage - 1) / kStage; }
+};
+
+// Grid: (feature tiles * C, token tiles); a cluster's C CTAs share a tile, each with
+// its slice of K.  Warp 0 loads, warp 1 multiplies, all four write out.
+template <int NT>
+__global__ void __launch_bounds__(128)
+skinny_kernel(const __grid_constant__ TmaArgs ta) {
+    using L = Skinny<NT>;
+    const Args& a = ta.a;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+    __shared__ uint32_t tmem_at;
+    const auto cluster = cooperative_groups::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t f0 = (int64_t)(blockIdx.x / C) * kFeatures, m0 = (int64_t)blockIdx.y * NT;
+    const int stages = ta.stages;
+    const int blocks = (int)((a.k + kBlockK - 1) / kBlockK);
+    const int kb0 = (int)((int64_t)blocks * rank / C), kb1 = (int)((int64_t)blocks * (rank + 1) / C);
+    const int nk = kb1 - kb0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            tc::mbar_init(tc::smem_u32(&full[s]), 1);
+            tc::mbar_init(tc::smem_u32(&empty[s]), 1);
+        }
+        tc::mbar_init(tc::smem_u32(&done), 1);
+        tc::fence_mbar_init();
+    }
+    if (warp == 1) tc::tmem_alloc(tc::smem_u32(&tmem_at), L::kTmem);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_at;
+    if (warp == 0 && lane == 0) {
+        for (int i = 0; i < nk; ++i) {
+            const int s = i % stages;
+            if (i >= stages && !tc::mbar_wait(tc::smem_u32(&empty[s]), (uint32_t)(i / stages - 1) & 1u)) {
+                report(a, 121);
+                break;
+            }
+            const uint32_t bar = tc::smem_u32(&full[s]), at = tc::smem_u32(smem + (size_t)s * L::kStage);
+            tc::mbar_expect_tx(bar, L::kStage);
+            tc::tma_load2(at, &ta.mw, (kb0 + i) * kBlockK, (int)f0, bar);
+            tc::tma_load2(at + kFeatures * kBlockK, &ta.mx, (kb0 + i) * kBlockK, (int)m0, bar);
+        }
+    } else if (warp == 1 && lane == 0) {
+        for (int i = 0; i < nk; ++i) {
+            const int s = i % stages;
+            if (!tc::mbar_wait(tc::smem_u32(&full[s]), (uint32_t)(i / stages) & 1u)) {
+                report(a, 122);
+                break;
+            }
+            tc::fence_after();
+            const uint32_t at = tc::smem_u32(smem + (size_t)s * L::kStage);
+            const uint64_t dw = sdesc_sw128(at), dx = sdesc_sw128(at + kFeatures * kBlockK);
+#pragma unroll
+            for (int j = 0; j < kBlockK / 32; ++j)          // 32 bytes of K an instruction: two 16-byte units
+                mma_i8(tmem, dw + 2 * j, dx + 2 * j, idesc_i8(kFeatures, NT), i || j);
+            tc::commit(tc::smem_u32(&empty[s]));
+        }
+        tc::commit(tc::smem_u32(&done));
+    }
+    __syncwarp();
+    const bool ok = tc::mbar_wait(tc::smem_u32(&done), 0);
+    if (!ok && lane == 0) report(a, 123);
+    tc::fence_after();
+    const int live = (int)min64(NT, a.tokens - m0);
+    const int64_t f = f0 + threadIdx.x;                     // this thread's feature: its lane of tensor memory
+    const bool in = f < a.features;
+    int* part = reinterpret_cast<int*>(smem);               // (token, feature of the tile)
+    const float ws = in ? a.ws[f] : 0.0f, bias = in && a.bias ? a.bias[f] : 0.0f;
+    auto put = [&](int m, int acc) {
+        const float v = fmaf((float)acc * a.xs[m0 + m], ws, bias);
+        if (in) st_any(a.out, (m0 + m) * a.features + f, a.out_dtype, v);
+    };
+    for (int c0 = 0; c0 < live; c0 += 16) {
+        int acc[16];
+        tmem_ld16(tmem + ((uint32_t)warp << 21) + c0, acc); // lanes 32 warp ..., columns c0 ...
+        wait_ld16(acc);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (c0 + j >= live) break;
+            if (C == 1) put(c0 + j, nk ? acc[j] : 0);
+            else part[(c0 + j) * kFeatures + threadIdx.x] = nk ? acc[j] : 0;
+        }
+    }
+    if (C > 1) {
+        cluster.sync();
+        // tokens rank, rank + C, ... of the tile: the slices added
+        for (int m = rank; m < live; m += C) {
+            int acc = 0;
+            for (int r = 0; r < C; ++r) acc += cluster.map_shared_rank(part, r)[m * kFeatures + threadIdx.x];
+            put(m, acc);
+        }
+        cluster.sync();
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 1) tc::tmem_dealloc(tmem, L::kTmem);
+}
+
+// Rows of K bytes at any stride to rows of `padded` bytes (a multiple of 16).
+__global__ void pack_kernel(const int8_t* src, int64_t stride, int8_t* dst, int64_t padded, int64_t rows, int64_t k) {
+    const int64_t words = padded / 4, n = rows * words;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / words, c = (i % words) * 4;
+        const int8_t* p = src + r * stride + c;
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < k) w |= (uint32_t)(uint8_t)p[j] << (8 * j);
+        *reinterpret_cast<uint32_t*>(dst + r * padded + c) = w;
+    }
+}
+
+// ------------------------------------------------------------------- host ----
+constexpr int64_t kMaxK = 131071;
+
+static bool al(const void* p, int64_t b) { return (reinterpret_cast<uintptr_t>(p) % b) == 0; }
+
+static int validate(const ssm_int8_linear_params* p) {
+    if (p == nullptr) return fail(SSM_ERR_INVALID, "int8_linear: null params");
+    if (p->tokens < 0 || p->in_features < 1 || p->out_features < 1)
+        return fail(SSM_ERR_INVALID, "int8_linear: tokens, in_features and out_features");
+    if (p->in_features > kMaxK)
+        return fail(SSM_ERR_UNSUPPORTED, "int8_linear: in_features above 131071 (the int32 sums could overflow)");
+    if (p->tokens > INT32_MAX || p->out_features > INT32_MAX)
+        return fail(SSM_ERR_UNSUPPORTED, "int8_linear: more than 2^31 - 1 tokens or out_features");
+    if (p->out_dtype < SSM_F32 || p->out_dtype > SSM_F16) return fail(SSM_ERR_UNSUPPORTED, "int8_linear: out_dtype");
+    if ((p->x_row_stride && p->x_row_stride < p->in_features) || (p->w_row_stride && p->w_row_stride < p->in_features))
+        return fail(SSM_ERR_INVALID, "int8_linear: a row stride is below in_features");
+    return SSM_OK;
+}
+
+static int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }
+static bool rows_ok(const void* p, int64_t stride, int64_t rows) {
+    return al(p, 16) && (rows == 1 || stride % 16 == 0) && stride < ((int64_t)1 << 40);
+}
+
+static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+        else
+            cudaGetLastError();
+    });
+    return fn;
+}
+
+static int encode(CUtensorMap* m, const void* base, int64_t k, int64_t rows, int64_t stride, int box_rows) {
+    if (!encoder()) return fail(SSM_ERR_CUDA, "int8_linear: cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(rows == 1 ? padded(k) : stride)};    // one row: never used
+    cuuint32_t box[2] = {kBlockK, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = encoder()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return SSM_OK;
+    return fail(SSM_ERR_CUDA, "int8_linear: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+}
+
+template <int NT>
+static int launch_skinny(TmaArgs& ta, cudaStream_t st) {
+    using L = Skinny<NT>;
+    const Args& a = ta.a;
+    const int64_t ftiles = ceil_div(a.features, kFeatures), mtiles = ceil_div(a.tokens, NT);
+    const int64_t blocks = ceil_div(a.k, kBlockK);
+    // K slices: until two CTAs per SM have work, at most eight, at least two blocks each
+    int C = 1;
+    while (C < 8 && ftiles * mtiles * (C + 1) <= 148 * 2 && blocks >= 2 * (C + 1)) ++C;
+    // the stages that let two CTAs share an SM, and hold the slices' sums
+    ta.stages = (int)max64(L::min_stages(), min64(min64(kMaxStages, ceil_div(blocks, C)), (110 << 10) / L::kStage));
+    const size_t smem = L::smem(ta.stages);
+    if (cudaFuncSetAttribute(skinny_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return check_launch("int8_linear");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(ftiles * C), (unsigned)mtiles);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, skinny_kernel<NT>, ta);
+    return check_launch("int8_linear");
+}
+
+}  // namespace i8
+}  // namespace ssm
+
+using namespace ssm;
+using namespace ssm::i8;
+
+// The kernels' error flag on the current device, read and cleared; called by
+// ssm_take_kernel_error.
+int ssm_i8_take_error() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, ssm::i8::g_i8_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(ssm::i8::g_i8_error, &zero, sizeof(int));
+    }
+    return v;
+}
+
+extern "C" int ssm_int8_linear_sizes(const ssm_int8_linear_params* p, size_t* workspace_bytes) {
+    if (int s = validate(p)) return s;
+    const int64_t xs = p->x_row_stride ? p->x_row_stride : p->in_features;
+    const int64_t ws = p->w_row_stride ? p->w_row_stride : p->in_features;
+    size_t need = 0;
+    if (!rows_ok(p->x, xs, p->tokens)) need += align_up((size_t)(p->tokens * padded(p->in_features)), 256);
+    if (!rows_ok(p->w, ws, p->out_features)) need += align_up((size_t)(p->out_features * padded(p->in_features)), 256);
+    if (workspace_bytes) *workspace_bytes = need;
+    return SSM_OK;
+}
+
+extern "C" int ssm_int8_linear_fwd(const ssm_int8_linear_params* p, void* stream) {
+    if (int s = validate(p)) return s;
+    if (p->tokens == 0) return SSM_OK;
+    if (!p->x || !p->x_scale || !p->w || !p->w_scale || !p->out)
+        return fail(SSM_ERR_INVALID, "int8_linear: null pointer");
+    size_t need = 0;
+    ssm_int8_linear_sizes(p, &need);
+    if (need && (!p->workspace || p->workspace_bytes < need || !al(p->workspace, 16)))
+        return fail(SSM_ERR_WORKSPACE, "int8_linear: workspace smaller than ssm_int8_linear_sizes");
+    if (int s = ensure_context("int8_linear")) return s;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int8_t* x = p->x;
+    const int8_t* w = p->w;
+    int64_t xs = p->x_row_stride ? p->x_row_stride : p->in_features;
+    int64_t ws = p->w_row_stride ? p->w_row_stride : p->in_features;
+    int8_t* room = static_cast<int8_t*>(p->workspace);
+    const int64_t k = p->in_features, kp = padded(k);
+    auto pack = [&](const int8_t*& src, int64_t& stride, int64_t rows) {
+        pack_kernel<<<(unsigned)min64(ceil_div(rows * kp / 4, 256), 148 * 16), 256, 0, st>>>(src, stride, room, kp, rows, k);
+        src = room;
+        stride = kp;
+        room += align_up((size_t)(rows * kp), 256);
+        return check_launch("int8_linear: pack");
+    };
+    if (!rows_ok(x, xs, p->tokens))
+        if (int s = pack(x, xs, p->tokens)) return s;
+    if (!rows_ok(w, ws, p->out_features))
+        if (int s = pack(w, ws, p->out_features)) return s;
+    TmaArgs ta{};
+    Args& a = ta.a;
+    a.tokens = p->tokens; a.features = p->out_features; a.k = k;
+    a.xs = p->x_scale; a.ws = p->w_scale; a.bias = p->bias;
+    a.out = p->out; a.out_dtype = p->out_dtype;
+    const int64_t es = p->out_dtype == SSM_F32 ? 4 : 2;
+    a.vec = al(p->out, 16) && (a.features * es) % 16 == 0;
+    a.status = p->status;
+    const int nt = a.tokens <= 16 ? 16 : a.tokens <= 32 ? 32 : a.tokens <= 64 ? 64 : 128;
+    if (int s = encode(&ta.mx, x, k, a.tokens, xs, nt)) return s;
+    if (int s = encode(&ta.mw, w, k, a.features, ws, kFeatures)) return s;
+    switch (nt) {
+        case 16: return launch_skinny<16>(ta, st);
+        case 32: return launch_skinny<32>(ta, st);
+        case 64: return launch_skinny<64>(ta, st);
+        default: return launch_skinny<128>(ta, st);
+    }
+}

@@ -1883,6 +1883,7 @@ __global__ void selftest_wait_kernel(int* status, uint32_t polls) {
 
 int ssm_conv_take_error();   // causal_conv1d.cu: the conv1d kernels' flag
 int ssm_glr_take_error();    // gated_recurrence.cu: the gated recurrence kernels' flag
+int ssm_i8_take_error();     // int8_linear.cu: the int8 linear layer's flag
 int ssm_scan_take_error();   // selective_scan_tma.cu: the TMA scan kernels' flag
 
 extern "C" int ssm_selftest_bounded_wait(int32_t* status, uint32_t polls, void* stream) {
@@ -1904,5 +1905,6 @@ extern "C" int ssm_take_kernel_error(void) {
     const int c = ssm_conv_take_error();
     const int sc = ssm_scan_take_error();
     const int gr = ssm_glr_take_error();
-    return v ? v : c ? c : sc ? sc : gr;
+    const int i8 = ssm_i8_take_error();
+    return v ? v : c ? c : sc ? sc : gr ? gr : i8;
 }

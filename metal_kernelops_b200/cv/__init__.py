@@ -13,6 +13,8 @@ Language-model operators around the scans (no counterpart in the reference):
 
 * ``add_rmsnorm``, ``add_rmsnorm_int8``, ``quantize_int8`` -- residual RMSNorm,
   its int8 output, and the row quantiser
+* ``int8_linear`` -- a linear layer on int8 rows with a scale per token and per
+  output feature
 * ``gated_linear_recurrence``, ``gated_linear_recurrence_update`` -- a diagonal
   recurrence with a forget gate per token: sequences (with gradients), one token
 
@@ -23,11 +25,12 @@ this package's scope.
 from .causal_conv1d import causal_conv1d_fn, causal_conv1d_update
 from .gated_norm import rmsnorm_gated
 from .gated_recurrence import gated_linear_recurrence, gated_linear_recurrence_update
+from .int8_matmul import int8_linear
 from .mamba2_chunk import last_path, mamba2_chunk_scan, tc_shape
 from .mamba2_state import mamba2_state_update
 from .path_scan import path_orders, ss2d_scan
 from .residual_norm import add_rmsnorm, add_rmsnorm_int8, quantize_int8
 
-__all__ = ["add_rmsnorm", "add_rmsnorm_int8", "quantize_int8", "causal_conv1d_fn", "causal_conv1d_update",
-           "gated_linear_recurrence", "gated_linear_recurrence_update", "last_path", "mamba2_chunk_scan",
-           "mamba2_state_update", "path_orders", "rmsnorm_gated", "ss2d_scan", "tc_shape"]
+__all__ = ["add_rmsnorm", "add_rmsnorm_int8", "causal_conv1d_fn", "causal_conv1d_update", "gated_linear_recurrence",
+           "gated_linear_recurrence_update", "int8_linear", "last_path", "mamba2_chunk_scan", "mamba2_state_update",
+           "path_orders", "quantize_int8", "rmsnorm_gated", "ss2d_scan", "tc_shape"]

@@ -53,3 +53,9 @@ def gated_recurrence_ref(x, forget, z=None, lower=None, init=None, reset=None):
     if z is not None:
         y = y * (z * torch.sigmoid(z))
     return y, h
+
+
+def int8_linear_ref(x, x_scale, weight, weight_scale, bias=None):
+    """The exact integer sums, scaled in float64."""
+    y = torch.matmul(x.double(), weight.double().t()) * x_scale.double()[..., None] * weight_scale.double()
+    return y if bias is None else y + bias.double()
