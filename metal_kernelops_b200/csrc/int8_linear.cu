@@ -13,6 +13,13 @@
 // the 128 rows of the product and the tokens its columns (16 to 128), and cuts K
 // over the CTAs of a cluster until the GPU is full; the slices' int32 sums are added
 // through distributed shared memory, exactly, so the cut changes no result.
+//
+// Many tokens: `wide_kernel`, a persistent pair of CTAs per 256 x 256 tile
+// (cta_group::2: each CTA loads 128 rows of either operand and keeps 128 token rows
+// of the sums).  A 128 x 256 tile on one CTA would fetch 96 bytes a clock from L2 to
+// feed its tensor core at the int8 rate, the pair fetches 64.  Warp-specialised: one
+// warp loads, one multiplies, four write the previous tile out from the other half
+// of tensor memory.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -35,7 +42,7 @@ struct Args {
     const float* xs; const float* ws; const float* bias;
     void* out;
     int out_dtype;
-    int vec;                                        // 16-byte stores are aligned
+    int vec;                                        // 32-byte stores are aligned
     int* status;
 };
 struct TmaArgs {
@@ -193,6 +200,234 @@ skinny_kernel(const __grid_constant__ TmaArgs ta) {
     if (warp == 1) tc::tmem_dealloc(tmem, L::kTmem);
 }
 
+// ----------------------------------------------------------- many tokens --
+constexpr int kTileM = 256, kTileN = 256;           // a CTA pair's tile
+constexpr int kWideStage = 2 * 128 * kBlockK;       // bytes a CTA stages: 128 token rows, 128 feature rows
+constexpr int kWideStages = 6;
+constexpr size_t kWideSmem = (size_t)kWideStages * kWideStage + 1024;
+constexpr int kWideThreads = 256;
+
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+// A load into this CTA's shared memory that counts its bytes on a barrier of the pair.
+__device__ __forceinline__ void pair_load(uint32_t dst, const void* map, int c0, int c1, uint32_t mbar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3}], [%4];"
+        :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(mbar) : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+        :: "r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+// Arrive on the barrier at this offset in both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void pair_commit(uint32_t mbar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        :: "r"(mbar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void st32(void* p, const uint32_t* w) {       // 32 bytes, 32-byte aligned
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+template <typename O> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 32 results of one token row at out + (columns f ... f + 31 of the features).
+template <typename O>
+__device__ __forceinline__ void write32(const Args& a, O* row, int64_t f, const float* v) {
+    if (f + 32 <= a.features && a.vec) {
+        uint32_t w[8];
+        constexpr int per = 32 / sizeof(O);
+#pragma unroll
+        for (int i = 0; i < 32; i += per) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (sizeof(O) == 4) w[j] = __float_as_uint(v[i + j]);
+                else w[j] = pack2<O>(v[i + 2 * j], v[i + 2 * j + 1]);
+            }
+            st32(row + f + i, w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (f + i < a.features) stf(row + f + i, v[i]);
+    }
+}
+
+template <typename O>
+__global__ void __launch_bounds__(kWideThreads, 1)
+wide_kernel(const __grid_constant__ TmaArgs ta) {
+    const Args& a = ta.a;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+    __shared__ uint64_t full[kWideStages], empty[kWideStages], tfull[2], tempty[2];
+    __shared__ __align__(16) float cols[2][kTileN];          // the tile's feature scales and biases
+    __shared__ uint32_t tmem_at;
+    const auto cluster = cooperative_groups::this_cluster();
+    const uint32_t rank = cluster.block_rank();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t mt = (a.tokens + kTileM - 1) / kTileM, nt = (a.features + kTileN - 1) / kTileN, tiles = mt * nt;
+    const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
+    const int nk = (int)((a.k + kBlockK - 1) / kBlockK);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kWideStages; ++s) {
+            tc::mbar_init(tc::smem_u32(&full[s]), 1);
+            tc::mbar_init(tc::smem_u32(&empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(tc::smem_u32(&tfull[b]), 1);
+            tc::mbar_init(tc::smem_u32(&tempty[b]), 8);      // four warps of either CTA
+        }
+        tc::fence_mbar_init();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;"
+                     :: "r"(tc::smem_u32(&tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc::fence_before();
+    cluster.sync();
+    tc::fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp == 0 && lane == 0) {
+        // loads: either CTA its own 128 rows of both operands, counted on the first CTA's barrier
+        int64_t it = 0;
+        bool ok = true;
+        for (int64_t tile = first; tile < tiles && ok; tile += step) {
+            const int m0 = (int)(tile / nt * kTileM + rank * 128), n0 = (int)(tile % nt * kTileN + rank * 128);
+            for (int kb = 0; kb < nk; ++kb, ++it) {
+                const int s = (int)(it % kWideStages);
+                if (it >= kWideStages &&
+                    !tc::mbar_wait(tc::smem_u32(&empty[s]), (uint32_t)(it / kWideStages - 1) & 1u)) {
+                    report(a, 131);
+                    ok = false;
+                    break;
+                }
+                const uint32_t bar = tc::smem_u32(&full[s]), at = tc::smem_u32(smem + (size_t)s * kWideStage);
+                if (rank == 0) tc::mbar_expect_tx(bar, 2 * kWideStage);
+                const uint32_t lead = at_rank(bar, 0);
+                pair_load(at, &ta.mx, kb * kBlockK, m0, lead);
+                pair_load(at + 128 * kBlockK, &ta.mw, kb * kBlockK, n0, lead);
+            }
+        }
+        // every stage's last use is over before the CTA may end
+        for (int64_t i = max64(0, it - kWideStages); ok && i < it; ++i)
+            if (!tc::mbar_wait(tc::smem_u32(&empty[i % kWideStages]), (uint32_t)(i / kWideStages) & 1u)) {
+                report(a, 132);
+                break;
+            }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        int64_t it = 0;
+        int64_t n = 0;
+        bool ok = true;
+        for (int64_t tile = first; tile < tiles && ok; tile += step, ++n) {
+            const int b = (int)(n & 1);
+            if (n >= 2 && !tc::mbar_wait(tc::smem_u32(&tempty[b]), (uint32_t)(n / 2 - 1) & 1u)) {
+                report(a, 133);
+                break;
+            }
+            tc::fence_after();
+            for (int kb = 0; kb < nk; ++kb, ++it) {
+                const int s = (int)(it % kWideStages);
+                if (!tc::mbar_wait(tc::smem_u32(&full[s]), (uint32_t)(it / kWideStages) & 1u)) {
+                    report(a, 134);
+                    ok = false;
+                    break;
+                }
+                tc::fence_after();
+                const uint32_t at = tc::smem_u32(smem + (size_t)s * kWideStage);
+                const uint64_t dx = sdesc_sw128(at), dw = sdesc_sw128(at + 128 * kBlockK);
+#pragma unroll
+                for (int j = 0; j < kBlockK / 32; ++j)
+                    pair_mma(tmem + b * kTileN, dx + 2 * j, dw + 2 * j, idesc_i8(kTileM, kTileN), kb || j);
+                pair_commit(tc::smem_u32(&empty[s]));
+            }
+            pair_commit(tc::smem_u32(&tfull[b]));
+        }
+    } else if (warp >= 4) {
+        // a wait that gave up is not tried again, so that the named barriers below stay in step
+        const int et = threadIdx.x - 128, ew = warp - 4;
+        int64_t n = 0;
+        bool ok = true;
+        for (int64_t tile = first; tile < tiles; tile += step, ++n) {
+            const int b = (int)(n & 1);
+            const int64_t m = tile / nt * kTileM + rank * 128 + et, n0 = tile % nt * kTileN;
+            asm volatile("bar.sync 1, 128;" ::: "memory");       // the previous tile's scales are read
+            for (int i = et; i < kTileN; i += 128) {
+                const int64_t f = n0 + i;
+                cols[0][i] = f < a.features ? a.ws[f] : 0.0f;
+                cols[1][i] = f < a.features && a.bias ? a.bias[f] : 0.0f;
+            }
+            const float xs = m < a.tokens ? a.xs[m] : 0.0f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (ok && !tc::mbar_wait(tc::smem_u32(&tfull[b]), (uint32_t)(n / 2) & 1u)) {
+                if (lane == 0) report(a, 135);
+                ok = false;
+            }
+            __syncwarp();
+            tc::fence_after();
+            O* row = static_cast<O*>(a.out) + m * a.features;
+#pragma unroll 1
+            for (int c0 = 0; c0 < kTileN; c0 += 32) {
+                int acc[32];
+                tmem_ld32(tmem + b * kTileN + c0 + ((uint32_t)ew << 21), acc);
+                wait_ld16(acc);
+                wait_ld16(acc + 16);
+                if (c0 + 32 == kTileN) {
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_at(at_rank(tc::smem_u32(&tempty[b]), 0));
+                }
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    const float4 w = *reinterpret_cast<const float4*>(&cols[0][c0 + i]);
+                    const float4 bb = *reinterpret_cast<const float4*>(&cols[1][c0 + i]);
+                    v[i] = fmaf((float)acc[i] * xs, w.x, bb.x);
+                    v[i + 1] = fmaf((float)acc[i + 1] * xs, w.y, bb.y);
+                    v[i + 2] = fmaf((float)acc[i + 2] * xs, w.z, bb.z);
+                    v[i + 3] = fmaf((float)acc[i + 3] * xs, w.w, bb.w);
+                }
+                if (m < a.tokens && ok) write32<O>(a, row, n0 + c0, v);
+            }
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    cluster.sync();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+}
+
 // Rows of K bytes at any stride to rows of `padded` bytes (a multiple of 16).
 __global__ void pack_kernel(const int8_t* src, int64_t stride, int8_t* dst, int64_t padded, int64_t rows, int64_t k) {
     const int64_t words = padded / 4, n = rows * words;
@@ -288,6 +523,30 @@ static int launch_skinny(TmaArgs& ta, cudaStream_t st) {
     return check_launch("int8_linear");
 }
 
+template <typename O>
+static int launch_wide(TmaArgs& ta, cudaStream_t st) {
+    const Args& a = ta.a;
+    const int64_t tiles = ceil_div(a.tokens, kTileM) * ceil_div(a.features, kTileN);
+    if (cudaFuncSetAttribute(wide_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWideSmem) != cudaSuccess)
+        return check_launch("int8_linear");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(2 * min64(tiles, 148 / 2)));
+    cfg.blockDim = dim3(kWideThreads);
+    cfg.dynamicSmemBytes = kWideSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, wide_kernel<O>, ta);
+    return check_launch("int8_linear");
+}
+
+// From this many tokens on the wide kernel runs.
+constexpr int64_t kWideTokens = 512;
+
 }  // namespace i8
 }  // namespace ssm
 
@@ -351,8 +610,14 @@ extern "C" int ssm_int8_linear_fwd(const ssm_int8_linear_params* p, void* stream
     a.xs = p->x_scale; a.ws = p->w_scale; a.bias = p->bias;
     a.out = p->out; a.out_dtype = p->out_dtype;
     const int64_t es = p->out_dtype == SSM_F32 ? 4 : 2;
-    a.vec = al(p->out, 16) && (a.features * es) % 16 == 0;
+    a.vec = al(p->out, 32) && (a.features * es) % 32 == 0;
     a.status = p->status;
+    if (a.tokens >= kWideTokens) {
+        if (int s = encode(&ta.mx, x, k, a.tokens, xs, 128)) return s;
+        if (int s = encode(&ta.mw, w, k, a.features, ws, 128)) return s;
+        if (p->out_dtype == SSM_F32) return launch_wide<float>(ta, st);
+        return p->out_dtype == SSM_BF16 ? launch_wide<__nv_bfloat16>(ta, st) : launch_wide<__half>(ta, st);
+    }
     const int nt = a.tokens <= 16 ? 16 : a.tokens <= 32 ? 32 : a.tokens <= 64 ? 64 : 128;
     if (int s = encode(&ta.mx, x, k, a.tokens, xs, nt)) return s;
     if (int s = encode(&ta.mw, w, k, a.features, ws, kFeatures)) return s;

@@ -101,7 +101,7 @@ def test_scales_that_are_zero_or_not_finite():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("offset", [0, 16, 5])
-@pytest.mark.parametrize("m", [7, 400])
+@pytest.mark.parametrize("m", [7, 400, 700])
 def test_strided_rows_leading_axes_and_another_stream(m, offset):
     """x and weight as column slices (aligned or not), on a stream of their own."""
     k, n = 320, 200
