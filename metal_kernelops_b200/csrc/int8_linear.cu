@@ -41,8 +41,7 @@ struct Args {
     int64_t tokens, features, k;
     const float* xs; const float* ws; const float* bias;
     void* out;
-    int out_dtype;
-    int vec;                                        // 32-byte stores are aligned
+    int vec, vec4;                                  // stores of 32 bytes, of four elements are aligned
     int* status;
 };
 struct TmaArgs {
@@ -90,19 +89,54 @@ __device__ __forceinline__ void wait_ld16(int* r) {
                  :: "memory");
 }
 
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ int4 ld_remote(uint32_t addr, uint32_t rank) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at_rank(addr, rank)) : "memory");
+    return v;
+}
+template <typename O> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four results of one token row.
+template <typename O>
+__device__ __forceinline__ void write4(const Args& a, O* row, int64_t f, float v0, float v1, float v2, float v3) {
+    if (f + 4 <= a.features && a.vec4) {
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<float4*>(row + f) = make_float4(v0, v1, v2, v3);
+        else *reinterpret_cast<uint2*>(row + f) = make_uint2(pack2<O>(v0, v1), pack2<O>(v2, v3));
+    } else {
+        if (f < a.features) stf(row + f, v0);
+        if (f + 1 < a.features) stf(row + f + 1, v1);
+        if (f + 2 < a.features) stf(row + f + 2, v2);
+        if (f + 3 < a.features) stf(row + f + 3, v3);
+    }
+}
+
 // ------------------------------------------------------------ few tokens --
 template <int NT>
 struct Skinny {
     static constexpr int kStage = kFeatures * kBlockK + NT * kBlockK;     // bytes: w rows, then x rows
     static constexpr uint32_t kTmem = NT < 32 ? 32 : NT;
     static size_t smem(int stages) { return (size_t)stages * kStage + 1024; }
-    // the K slices' sums meet in the stages' memory
+    // the sums pass through the stages' memory
     static int min_stages() { return (NT * kFeatures * 4 + kStage - 1) / kStage; }
 };
 
 // Grid: (feature tiles * C, token tiles); a cluster's C CTAs share a tile, each with
 // its slice of K.  Warp 0 loads, warp 1 multiplies, all four write out.
-template <int NT>
+template <typename O, int NT>
 __global__ void __launch_bounds__(128)
 skinny_kernel(const __grid_constant__ TmaArgs ta) {
     using L = Skinny<NT>;
@@ -119,6 +153,13 @@ skinny_kernel(const __grid_constant__ TmaArgs ta) {
     const int blocks = (int)((a.k + kBlockK - 1) / kBlockK);
     const int kb0 = (int)((int64_t)blocks * rank / C), kb1 = (int)((int64_t)blocks * (rank + 1) / C);
     const int nk = kb1 - kb0;
+    auto load = [&](int i) {
+        const int s = i % stages;
+        const uint32_t bar = tc::smem_u32(&full[s]), at = tc::smem_u32(smem + (size_t)s * L::kStage);
+        tc::mbar_expect_tx(bar, L::kStage);
+        tc::tma_load2(at, &ta.mw, (kb0 + i) * kBlockK, (int)f0, bar);
+        tc::tma_load2(at + kFeatures * kBlockK, &ta.mx, (kb0 + i) * kBlockK, (int)m0, bar);
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             tc::mbar_init(tc::smem_u32(&full[s]), 1);
@@ -126,6 +167,8 @@ skinny_kernel(const __grid_constant__ TmaArgs ta) {
         }
         tc::mbar_init(tc::smem_u32(&done), 1);
         tc::fence_mbar_init();
+        // the ring's first loads go out before the CTA has its tensor memory
+        for (int i = 0; i < stages && i < nk; ++i) load(i);
     }
     if (warp == 1) tc::tmem_alloc(tc::smem_u32(&tmem_at), L::kTmem);
     tc::fence_before();
@@ -133,16 +176,12 @@ skinny_kernel(const __grid_constant__ TmaArgs ta) {
     tc::fence_after();
     const uint32_t tmem = tmem_at;
     if (warp == 0 && lane == 0) {
-        for (int i = 0; i < nk; ++i) {
-            const int s = i % stages;
-            if (i >= stages && !tc::mbar_wait(tc::smem_u32(&empty[s]), (uint32_t)(i / stages - 1) & 1u)) {
+        for (int i = stages; i < nk; ++i) {
+            if (!tc::mbar_wait(tc::smem_u32(&empty[i % stages]), (uint32_t)(i / stages - 1) & 1u)) {
                 report(a, 121);
                 break;
             }
-            const uint32_t bar = tc::smem_u32(&full[s]), at = tc::smem_u32(smem + (size_t)s * L::kStage);
-            tc::mbar_expect_tx(bar, L::kStage);
-            tc::tma_load2(at, &ta.mw, (kb0 + i) * kBlockK, (int)f0, bar);
-            tc::tma_load2(at + kFeatures * kBlockK, &ta.mx, (kb0 + i) * kBlockK, (int)m0, bar);
+            load(i);
         }
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < nk; ++i) {
@@ -165,36 +204,45 @@ skinny_kernel(const __grid_constant__ TmaArgs ta) {
     const bool ok = tc::mbar_wait(tc::smem_u32(&done), 0);
     if (!ok && lane == 0) report(a, 123);
     tc::fence_after();
+    // tensor memory (lane: feature, column: token) to shared memory (token, feature)
     const int live = (int)min64(NT, a.tokens - m0);
-    const int64_t f = f0 + threadIdx.x;                     // this thread's feature: its lane of tensor memory
-    const bool in = f < a.features;
-    int* part = reinterpret_cast<int*>(smem);               // (token, feature of the tile)
-    const float ws = in ? a.ws[f] : 0.0f, bias = in && a.bias ? a.bias[f] : 0.0f;
-    auto put = [&](int m, int acc) {
-        const float v = fmaf((float)acc * a.xs[m0 + m], ws, bias);
-        if (in) st_any(a.out, (m0 + m) * a.features + f, a.out_dtype, v);
-    };
+    int* part = reinterpret_cast<int*>(smem);
     for (int c0 = 0; c0 < live; c0 += 16) {
         int acc[16];
         tmem_ld16(tmem + ((uint32_t)warp << 21) + c0, acc); // lanes 32 warp ..., columns c0 ...
         wait_ld16(acc);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            if (c0 + j >= live) break;
-            if (C == 1) put(c0 + j, nk ? acc[j] : 0);
-            else part[(c0 + j) * kFeatures + threadIdx.x] = nk ? acc[j] : 0;
-        }
+        for (int j = 0; j < 16; ++j)
+            if (c0 + j < live) part[(c0 + j) * kFeatures + threadIdx.x] = acc[j];
     }
-    if (C > 1) {
-        cluster.sync();
-        // tokens rank, rank + C, ... of the tile: the slices added
-        for (int m = rank; m < live; m += C) {
-            int acc = 0;
-            for (int r = 0; r < C; ++r) acc += cluster.map_shared_rank(part, r)[m * kFeatures + threadIdx.x];
-            put(m, acc);
-        }
-        cluster.sync();
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+    // a thread: four features of every (4 C)-th token, the slices of K added
+    const int64_t f = f0 + lane * 4;
+    float ws[4], bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        ws[j] = f + j < a.features ? a.ws[f + j] : 0.0f;
+        bias[j] = f + j < a.features && a.bias ? a.bias[f + j] : 0.0f;
     }
+    const uint32_t mine = tc::smem_u32(part + lane * 4);
+#pragma unroll 2
+    for (int m = rank * 4 + warp; m < live; m += 4 * C) {
+        const float xs = a.xs[m0 + m];
+        int4 v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            v[r] = make_int4(0, 0, 0, 0);
+            if (r < C) v[r] = ld_remote(mine + m * kFeatures * 4, r);
+        }
+        int4 s = v[0];
+#pragma unroll
+        for (int r = 1; r < 8; ++r) { s.x += v[r].x; s.y += v[r].y; s.z += v[r].z; s.w += v[r].w; }
+        write4<O>(a, static_cast<O*>(a.out) + (m0 + m) * a.features, f, fmaf((float)s.x * xs, ws[0], bias[0]),
+                  fmaf((float)s.y * xs, ws[1], bias[1]), fmaf((float)s.z * xs, ws[2], bias[2]),
+                  fmaf((float)s.w * xs, ws[3], bias[3]));
+    }
+    if (C > 1) cluster.sync();                              // the peers have read this CTA's sums
     tc::fence_before();
     __syncthreads();
     if (warp == 1) tc::tmem_dealloc(tmem, L::kTmem);
@@ -207,11 +255,6 @@ constexpr int kWideStages = 6;
 constexpr size_t kWideSmem = (size_t)kWideStages * kWideStage + 1024;
 constexpr int kWideThreads = 256;
 
-__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 // A load into this CTA's shared memory that counts its bytes on a barrier of the pair.
 __device__ __forceinline__ void pair_load(uint32_t dst, const void* map, int c0, int c1, uint32_t mbar) {
     asm volatile(
@@ -251,16 +294,6 @@ __device__ __forceinline__ void st32(void* p, const uint32_t* w) {       // 32 b
                  :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
 }
-template <typename O> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // 32 results of one token row at out + (columns f ... f + 31 of the features).
 template <typename O>
 __device__ __forceinline__ void write32(const Args& a, O* row, int64_t f, const float* v) {
@@ -494,7 +527,7 @@ static int encode(CUtensorMap* m, const void* base, int64_t k, int64_t rows, int
     return fail(SSM_ERR_CUDA, "int8_linear: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
 }
 
-template <int NT>
+template <typename O, int NT>
 static int launch_skinny(TmaArgs& ta, cudaStream_t st) {
     using L = Skinny<NT>;
     const Args& a = ta.a;
@@ -503,10 +536,10 @@ static int launch_skinny(TmaArgs& ta, cudaStream_t st) {
     // K slices: until two CTAs per SM have work, at most eight, at least two blocks each
     int C = 1;
     while (C < 8 && ftiles * mtiles * (C + 1) <= 148 * 2 && blocks >= 2 * (C + 1)) ++C;
-    // the stages that let two CTAs share an SM, and hold the slices' sums
+    // the stages that let two CTAs share an SM, and hold the sums
     ta.stages = (int)max64(L::min_stages(), min64(min64(kMaxStages, ceil_div(blocks, C)), (110 << 10) / L::kStage));
     const size_t smem = L::smem(ta.stages);
-    if (cudaFuncSetAttribute(skinny_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    if (cudaFuncSetAttribute(skinny_kernel<O, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return check_launch("int8_linear");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(ftiles * C), (unsigned)mtiles);
@@ -519,8 +552,18 @@ static int launch_skinny(TmaArgs& ta, cudaStream_t st) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, skinny_kernel<NT>, ta);
+    cudaLaunchKernelEx(&cfg, skinny_kernel<O, NT>, ta);
     return check_launch("int8_linear");
+}
+
+template <typename O>
+static int launch_few(TmaArgs& ta, int nt, cudaStream_t st) {
+    switch (nt) {
+        case 16: return launch_skinny<O, 16>(ta, st);
+        case 32: return launch_skinny<O, 32>(ta, st);
+        case 64: return launch_skinny<O, 64>(ta, st);
+        default: return launch_skinny<O, 128>(ta, st);
+    }
 }
 
 template <typename O>
@@ -608,9 +651,10 @@ extern "C" int ssm_int8_linear_fwd(const ssm_int8_linear_params* p, void* stream
     Args& a = ta.a;
     a.tokens = p->tokens; a.features = p->out_features; a.k = k;
     a.xs = p->x_scale; a.ws = p->w_scale; a.bias = p->bias;
-    a.out = p->out; a.out_dtype = p->out_dtype;
+    a.out = p->out;
     const int64_t es = p->out_dtype == SSM_F32 ? 4 : 2;
     a.vec = al(p->out, 32) && (a.features * es) % 32 == 0;
+    a.vec4 = al(p->out, 4 * es) && a.features % 4 == 0;
     a.status = p->status;
     if (a.tokens >= kWideTokens) {
         if (int s = encode(&ta.mx, x, k, a.tokens, xs, 128)) return s;
@@ -621,10 +665,6 @@ extern "C" int ssm_int8_linear_fwd(const ssm_int8_linear_params* p, void* stream
     const int nt = a.tokens <= 16 ? 16 : a.tokens <= 32 ? 32 : a.tokens <= 64 ? 64 : 128;
     if (int s = encode(&ta.mx, x, k, a.tokens, xs, nt)) return s;
     if (int s = encode(&ta.mw, w, k, a.features, ws, kFeatures)) return s;
-    switch (nt) {
-        case 16: return launch_skinny<16>(ta, st);
-        case 32: return launch_skinny<32>(ta, st);
-        case 64: return launch_skinny<64>(ta, st);
-        default: return launch_skinny<128>(ta, st);
-    }
+    if (p->out_dtype == SSM_F32) return launch_few<float>(ta, nt, st);
+    return p->out_dtype == SSM_BF16 ? launch_few<__nv_bfloat16>(ta, nt, st) : launch_few<__half>(ta, nt, st);
 }
