@@ -527,17 +527,52 @@ static int encode(CUtensorMap* m, const void* base, int64_t k, int64_t rows, int
     return fail(SSM_ERR_CUDA, "int8_linear: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
 }
 
+// How many clusters of C CTAs with S stages each the GPU holds at once.  The
+// occupancy query counts kernels that allocate tensor memory as one CTA an SM; shared
+// and tensor memory say how many more share it.
+template <typename O, int NT>
+static int64_t clusters_at_once(int S, int C) {
+    static int alone[9];                             // with one CTA an SM; 0: not asked yet
+    if (alone[C] == 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(C);
+        cfg.blockDim = dim3(128);
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = C;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, skinny_kernel<O, NT>, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 128 / C;
+        }
+        alone[C] = n;
+    }
+    // 228 KB an SM; a CTA also has its barriers and 1 KB of the system's
+    const int64_t by_smem = (228 << 10) / (int64_t)(Skinny<NT>::smem(S) + 2048);
+    return alone[C] * max64(1, min64(by_smem, 512 / Skinny<NT>::kTmem));
+}
+
 template <typename O, int NT>
 static int launch_skinny(TmaArgs& ta, cudaStream_t st) {
     using L = Skinny<NT>;
     const Args& a = ta.a;
     const int64_t ftiles = ceil_div(a.features, kFeatures), mtiles = ceil_div(a.tokens, NT);
     const int64_t blocks = ceil_div(a.k, kBlockK);
-    // K slices: until two CTAs per SM have work, at most eight, at least two blocks each
-    int C = 1;
-    while (C < 8 && ftiles * mtiles * (C + 1) <= 148 * 2 && blocks >= 2 * (C + 1)) ++C;
-    // the stages that let two CTAs share an SM, and hold the sums
-    ta.stages = (int)max64(L::min_stages(), min64(min64(kMaxStages, ceil_div(blocks, C)), (110 << 10) / L::kStage));
+    // As many K slices as let every cluster run at once (at most eight, at least two
+    // blocks each), with about 72 KB of stages a CTA; then more stages while all still
+    // fit.  One cluster too many costs a second wave: 1 x 2560 -> 12368 takes 10.1 us with
+    // three slices of four stages, 14.9 us with six stages, of which one of the 97
+    // clusters has to wait; 11.5 us uncut.
+    const int64_t tiles = ftiles * mtiles;
+    auto fits = [&](int s, int c) { return tiles <= clusters_at_once<O, NT>(s, c); };
+    const int least = (int)max64(L::min_stages(), 2);
+    int S = (int)max64(least, (72 << 10) / L::kStage), C = 1;
+    while (C < 8 && blocks >= 2 * (C + 1) && fits(S, C + 1)) ++C;
+    while (S < kMaxStages && (int64_t)S * C < blocks && (size_t)(S + 1) * L::kStage <= (200 << 10) && fits(S + 1, C)) ++S;
+    ta.stages = S;
     const size_t smem = L::smem(ta.stages);
     if (cudaFuncSetAttribute(skinny_kernel<O, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return check_launch("int8_linear");
@@ -587,8 +622,9 @@ static int launch_wide(TmaArgs& ta, cudaStream_t st) {
     return check_launch("int8_linear");
 }
 
-// From this many tokens on the wide kernel runs.
-constexpr int64_t kWideTokens = 512;
+// From this many tokens on the wide kernel runs: at 256 x 2560 -> 12368 the skinny one
+// takes 20.7 us and the wide one 21.5, at 400 28.0 and 21.6.
+constexpr int64_t kWideTokens = 257;
 
 }  // namespace i8
 }  // namespace ssm

@@ -45,11 +45,12 @@ def _forward(x, x_scale, weight, weight_scale, bias, out_dtype):
     features, k = weight.shape
     dev = x.device
     out = torch.empty((*x.shape[:-1], features), dtype=out_dtype, device=dev)
+    xp, wp, xr, wr = x.data_ptr(), weight.data_ptr(), _stride(x), _stride(weight)
     p = nat.Int8LinearParams(
-        x.numel() // k, k, features, _stride(x), _stride(weight), nat.dtype_code(out_dtype), 0, x.data_ptr(),
-        x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-        out.data_ptr(), None, 0, nat.status_word(dev, "int8_linear"))
-    if k % 16 or x.data_ptr() % 16 or weight.data_ptr() % 16 or p.x_row_stride % 16 or p.w_row_stride % 16:
+        x.numel() // k, k, features, xr, wr, nat.dtype_code(out_dtype), 0, xp, x_scale.data_ptr(), wp,
+        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), None, 0,
+        nat.status_word(dev, "int8_linear"))
+    if (k | xp | wp | xr | wr) % 16:
         need = nat._SZ()
         nat.check(nat.lib().ssm_int8_linear_sizes(p, need), "int8_linear")
         ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=dev)
@@ -83,31 +84,30 @@ def int8_linear(x, x_scale, weight, weight_scale, bias=None, out_dtype=torch.bfl
     Returns:
         ``(..., out_features)`` in ``out_dtype``.
     """
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
-        raise ValueError(f"int8_linear: x (..., in) and weight (out, in), got {tuple(x.shape)} and {tuple(weight.shape)}")
+    shape, wshape = x.shape, weight.shape
+    if len(shape) < 1 or len(wshape) != 2 or shape[-1] != wshape[1] or 0 in wshape:
+        raise ValueError(f"int8_linear: x (..., in) and weight (out, in), got {tuple(shape)} and {tuple(wshape)}")
     if x.dtype is not torch.int8 or weight.dtype is not torch.int8:
         raise ValueError(f"int8_linear: x and weight are int8, got {x.dtype} and {weight.dtype}")
-    if x_scale.shape != x.shape[:-1] or weight_scale.shape != weight.shape[:1]:
-        raise ValueError(f"int8_linear: x_scale must be {tuple(x.shape[:-1])} and weight_scale {tuple(weight.shape[:1])}, "
+    if x_scale.shape != shape[:-1] or weight_scale.shape != wshape[:1]:
+        raise ValueError(f"int8_linear: x_scale must be {tuple(shape[:-1])} and weight_scale {tuple(wshape[:1])}, "
                          f"got {tuple(x_scale.shape)} and {tuple(weight_scale.shape)}")
     if x_scale.dtype is not torch.float32 or weight_scale.dtype is not torch.float32:
         raise ValueError(f"int8_linear: the scales are float32, got {x_scale.dtype} and {weight_scale.dtype}")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError(f"int8_linear: bias must be {tuple(weight.shape[:1])}, got {tuple(bias.shape)}")
+    if bias is not None and bias.shape != wshape[:1]:
+        raise ValueError(f"int8_linear: bias must be {tuple(wshape[:1])}, got {tuple(bias.shape)}")
     if out_dtype not in _DTYPES:
         raise ValueError(f"int8_linear: out_dtype is float32/bfloat16/float16, got {out_dtype}")
-    index = x.get_device()
+    index = x.get_device()                          # negative off the GPU
     for label, t in (("x", x), ("x_scale", x_scale), ("weight", weight), ("weight_scale", weight_scale), ("bias", bias)):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"int8_linear runs CUDA kernels, {label} is on {t.device}")
-        if t.get_device() != index:
+        if t is not None and (index < 0 or t.get_device() != index):
+            if not t.is_cuda:
+                raise ValueError(f"int8_linear runs CUDA kernels, {label} is on {t.device}")
             raise ValueError(f"int8_linear: {label} is on {t.device}, x is on {x.device}")
     if nat.wants_grad(x_scale, weight_scale, bias):
         raise ValueError("int8_linear has no gradient: call it under torch.no_grad()")
-    if x.numel() == 0:
-        return torch.empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype, device=x.device)
+    if 0 in shape:
+        return torch.empty((*shape[:-1], wshape[0]), dtype=out_dtype, device=x.device)
     x, weight = _rows(x), _rows(weight)
     if not x_scale.is_contiguous():
         x_scale = x_scale.contiguous()

@@ -193,13 +193,13 @@ def _check(name, x, weight, residual):
         raise ValueError(f"weight must be ({shape[-1]},), got {tuple(weight.shape)}")
     if residual is not None and residual.shape != shape:
         raise ValueError(f"residual must match x {tuple(shape)}, got {tuple(residual.shape)}")
-    index = x.get_device()
+    index = x.get_device()                          # negative off the GPU
     for label, t in (("x", x), ("weight", weight), ("residual", residual)):
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} runs CUDA kernels, {label} is on {t.device}")
-        if t.get_device() != index:
+        if index < 0 or t.get_device() != index:
+            if not t.is_cuda:
+                raise ValueError(f"{name} runs CUDA kernels, {label} is on {t.device}")
             raise ValueError(f"{name}: {label} is on {t.device}, x is on {x.device}")
         if t.dtype not in _DTYPES:
             raise ValueError(f"{name} computes float32/bfloat16/float16, {label} is {t.dtype}")
