@@ -163,6 +163,23 @@ __device__ __forceinline__ void st_word(T* p, typename Lane<T>::F v, int64_t c, 
         }
     }
 }
+// The lane's words of one output tensor, step by step.  ODD: words may be unaligned or
+// half outside; otherwise one predicated 4-byte store.
+template <typename T, bool ODD>
+struct Out {
+    T* p;
+    int live;                                       // steps to store: none for channels outside
+    int64_t c, dim;
+    __device__ __forceinline__ Out(void* base, int64_t at, int64_t c_, int64_t dim_, int n)
+        : p(static_cast<T*>(base) + at), live(c_ < dim_ ? n : 0), c(c_), dim(dim_) {}
+    __device__ __forceinline__ void put(int i, typename Lane<T>::F v) const {
+        if (i < live) {
+            if constexpr (ODD) st_word<T>(p, v, c, dim, false);
+            else st_lane(p, v);
+        }
+    }
+    __device__ __forceinline__ void move(int64_t by) { p += by; }
+};
 // The lane's channels of a per-channel fp32 array; `none` where absent or outside.
 __device__ __forceinline__ void ld_chan(const float* p, int64_t c, int64_t dim, float none, float& v) {
     v = (p != nullptr && c < dim) ? p[c] : none;
@@ -437,8 +454,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
         // the state that enters every kBwdSteps kWarps steps, for the backward
         if (a.states != nullptr && warp % (kBwdSteps * kWarps / N) == 0 && live > 0)
             st_chan(a.states + (b * a.saved + t / (kBwdSteps * kWarps)) * a.dim, c, a.dim, h);
-        T* y = static_cast<T*>(a.y) + (b * a.length + t) * a.dim + c;
-        const bool whole = live == N && a.words && c + E <= a.dim;
+        Out<T, LOADS == kDirect> y(a.y, (b * a.length + t) * a.dim + c, c, a.dim, live);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (RESET && (rs >> i & 1u)) h = same<F>(0.0f);
@@ -448,8 +464,8 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
                 const F z = unpack<T>(zw[i]);
                 o = mu(h, mu(z, sigmoid_pos(z)));
             }
-            if (whole) st_lane(y + i * a.dim, o);
-            else if (i < live) st_word<T>(y + i * a.dim, o, c, a.dim, a.words);
+            y.put(i, o);
+            y.move(a.dim);
         }
     }
     if (C > 1) cluster.sync();                          // nothing is on its way to a CTA that ends
@@ -608,13 +624,9 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         again(k);
         again(dw);
         if (GATE) again(zw);
-        const int64_t at = (b * a.length + t) * a.dim + c;
-        const bool whole = live == N && a.words && c + E <= a.dim;
-        auto put = [&](void* base, int i, F v) {
-            T* p = static_cast<T*>(base) + at + i * a.dim;
-            if (whole) st_lane(p, v);
-            else if (i < live) st_word<T>(p, v, c, a.dim, a.words);
-        };
+        const int64_t at = (b * a.length + t + N - 1) * a.dim + c;
+        Out<T, LOADS == kDirect> dx(a.dx, at, c, a.dim, live), df(a.dforget, at, c, a.dim, live);
+        Out<T, LOADS == kDirect> dz(GATE ? a.dz : nullptr, at, c, a.dim, live);
         F dl = zero;
 #pragma unroll
         for (int i = N - 1; i >= 0; --i) {
@@ -625,12 +637,15 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 e = mu(dy, zs);
                 // silu'(z) = s + z s (1 - s)
                 const F ds = fm(zs, sub(one, s), s);
-                put(a.dz, i, mu(mu(dy, fm(av, hp[i], mu(g, x))), ds));
+                dz.put(i, mu(mu(dy, fm(av, hp[i], mu(g, x))), ds));
+                dz.move(-a.dim);
             }
             d = ad(d, e);                          // dh of step i
             const F dg = mu(d, sub(x, hp[i]));
-            put(a.dx, i, mu(g, d));
-            put(a.dforget, i, mu(mu(dg, g), sub(k[i], one)));
+            dx.put(i, mu(g, d));
+            dx.move(-a.dim);
+            df.put(i, mu(mu(dg, g), sub(k[i], one)));
+            df.move(-a.dim);
             dl = fm(dg, k[i], dl);
             d = mu(d, av);
             if (RESET && (rs >> i & 1u)) d = zero;
@@ -874,7 +889,7 @@ static int launch_any(const ssm_gated_recurrence_params* p, const Args& a, bool 
     TmaArgs ta{};
     ta.a = a;
     const bool tma = tma_ok(a, p->dtype, bwd);
-    const int loads = tma ? kTma : a.words ? kWords : kDirect;
+    const int loads = !a.words ? kDirect : tma ? kTma : kWords;
     const int chunk = kWarps * (bwd ? kBwdSteps : kFwdSteps);
     if (tma) {
         if (int s = ensure_context("gated_linear_recurrence")) return s;
