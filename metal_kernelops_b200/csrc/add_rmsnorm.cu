@@ -411,22 +411,25 @@ bwd_stream_kernel(const Args a) {
     }
 }
 
-// dw[f] = the partial rows added in order: 32 columns a CTA, eight runs of
-// consecutive partial rows each summed by one warp, the runs added in order.
-__global__ void __launch_bounds__(256) fold_kernel(const float* part, int64_t parts, int64_t F, float* dw) {
-    __shared__ float run[8][32];
+// dw[f] = the partial rows added in order: 32 columns a CTA, 32 runs of consecutive
+// partial rows each summed by one warp, the runs added in order.
+constexpr int kRuns = 32;
+__global__ void __launch_bounds__(kRuns * 32) fold_kernel(const float* part, int64_t parts, int64_t F, float* dw) {
+    __shared__ float run[kRuns][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t f = (int64_t)blockIdx.x * 32 + lane;
-    const int64_t per = (parts + 7) / 8, k0 = warp * per, k1 = min64(k0 + per, parts);
+    const int64_t per = (parts + kRuns - 1) / kRuns, k0 = warp * per, k1 = min64(k0 + per, parts);
     float s = 0.0f;
-    if (f < F)
+    if (f < F) {
+#pragma unroll 8
         for (int64_t k = k0; k < k1; ++k) s += part[k * F + f];
+    }
     run[warp][lane] = s;
     __syncthreads();
     if (warp == 0 && f < F) {
         s = run[0][lane];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += run[i][lane];
+        for (int i = 1; i < kRuns; ++i) s += run[i][lane];
         dw[f] = s;
     }
 }
@@ -437,17 +440,20 @@ static int64_t esize(int dtype) { return dtype == SSM_F32 ? 4 : 2; }
 
 // v elements a vector (8, or 1 where width or alignment does not allow 8), nv
 // vectors a thread, tx threads a row, ty rows a CTA; nv = 0: the streaming
-// kernels.  Rows of up to 512 vectors take one vector a thread (v = 8).
+// kernels.  The forward gives a thread four vectors where the row has them: with
+// 65536 x 2560 bf16 to int8, 177 us against 189 with two and 219 with one (fewer
+// warps meet at the reduction, each with more loads on the way).  The backward,
+// which keeps three tensors' vectors, weights and sums, takes one: 505 us, 520 with
+// two and 1592 (spilled) with four.
 struct Shape { int tx, ty, v, nv; };
 
 static Shape shape_of(int64_t F, bool vec, bool bwd) {
     const int v = vec ? 8 : 1;
     const int64_t n = ceil_div(F, v);
     int nv = 0;
-    for (int c : {1, 2, 4})
-        if (vec && nv == 0 && n <= (int64_t)c * kMaxThreads && !(bwd && c == 4)) nv = c;
-    for (int c : {8, 16})
-        if (!vec && nv == 0 && n <= (int64_t)c * kMaxThreads) nv = c;
+    if (vec && bwd) nv = n <= kMaxThreads ? 1 : n <= 2 * kMaxThreads ? 2 : 0;
+    else if (vec) nv = n <= 32 ? 1 : n <= 64 ? 2 : n <= 4 * kMaxThreads ? 4 : 0;
+    else nv = n <= 8 * kMaxThreads ? 8 : n <= 16 * kMaxThreads ? 16 : 0;
     if (nv == 0) return {kMaxThreads, 1, 1, 0};
     const int tx = (int)(ceil_div(ceil_div(n, nv), 32) * 32);
     return {tx, tx >= 128 ? 1 : 128 / tx, v, nv};
@@ -518,18 +524,37 @@ static bool vec_fwd(const ssm_add_rmsnorm_params* p, const Args& a, bool quant_o
     return !a.res || (al(a.res, 16) && (a.rs * es) % 16 == 0 && al(a.stream, 16));
 }
 
-// Backward CTAs: rows in turn over up to two CTAs per SM.
-static int64_t bwd_ctas(int64_t rows, int ty) { return min64(ceil_div(max64(rows, 1), ty), 148 * 2); }
+// The most CTAs the backward runs (each leaves ty partial rows): 1024 threads an SM.
+static int64_t most_ctas(int64_t rows, const Shape& s) {
+    return min64(ceil_div(max64(rows, 1), s.ty), 148 * max64(1, 1024 / (s.tx * s.ty)));
+}
+// As many of them as the GPU holds at once.
+template <auto kernel>
+static int64_t launch_rows(Args& a, const Shape& s, cudaStream_t st) {
+    static int room[kMaxThreads / 32 + 1];            // CTAs per SM by warps; 0: not asked yet
+    int& n = room[s.tx * s.ty / 32];
+    if (n == 0) {
+        int k = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&k, kernel, s.tx * s.ty, 0) != cudaSuccess || k < 1) {
+            cudaGetLastError();
+            k = 1;
+        }
+        n = k;
+    }
+    const int64_t ctas = min64(most_ctas(a.rows, s), 148 * n);
+    kernel<<<(unsigned)ctas, dim3(s.tx, s.ty), 0, st>>>(a);
+    return ctas;
+}
 
+// Returns the CTAs launched.
 template <typename T, typename TS>
-static void launch_bwd(const Args& a, const Shape& s, int64_t ctas, cudaStream_t st) {
-    const dim3 block(s.tx, s.ty);
+static int64_t launch_bwd(Args& a, const Shape& s, cudaStream_t st) {
     switch (s.nv) {
-        case 0: bwd_stream_kernel<T, TS><<<(unsigned)ctas, block, 0, st>>>(a); break;
-        case 1: bwd_kernel<T, TS, 8, 1><<<(unsigned)ctas, block, 0, st>>>(a); break;
-        case 2: bwd_kernel<T, TS, 8, 2><<<(unsigned)ctas, block, 0, st>>>(a); break;
-        case 8: bwd_kernel<T, TS, 1, 8><<<(unsigned)ctas, block, 0, st>>>(a); break;
-        default: bwd_kernel<T, TS, 1, 16><<<(unsigned)ctas, block, 0, st>>>(a);
+        case 0: return launch_rows<bwd_stream_kernel<T, TS>>(a, s, st);
+        case 1: return launch_rows<bwd_kernel<T, TS, 8, 1>>(a, s, st);
+        case 2: return launch_rows<bwd_kernel<T, TS, 8, 2>>(a, s, st);
+        case 8: return launch_rows<bwd_kernel<T, TS, 1, 8>>(a, s, st);
+        default: return launch_rows<bwd_kernel<T, TS, 1, 16>>(a, s, st);
     }
 }
 
@@ -545,7 +570,7 @@ extern "C" int ssm_add_rmsnorm_sizes(const ssm_add_rmsnorm_params* p, size_t* wo
     int64_t parts = 0;
     for (bool vec : {false, true}) {
         const Shape sh = shape_of(p->features, vec && p->features % 8 == 0, true);
-        parts = max64(parts, bwd_ctas(p->rows, sh.ty) * sh.ty);
+        parts = max64(parts, most_ctas(p->rows, sh) * sh.ty);
     }
     if (workspace_bytes) *workspace_bytes = (size_t)(parts * p->features) * 4;
     return SSM_OK;
@@ -595,15 +620,15 @@ extern "C" int ssm_add_rmsnorm_bwd(const ssm_add_rmsnorm_params* p, void* stream
                      al(a.dy, 16) && (a.dys * e) % 16 == 0 && al(a.dx, 16) && al(a.part, 16) &&
                      (!a.ds || (al(a.ds, 16) && (a.dss * es) % 16 == 0)) && (!a.dres || al(a.dres, 16));
     const Shape sh = shape_of(a.features, vec, true);
-    const int64_t ctas = bwd_ctas(a.rows, sh.ty);
-    if (p->dtype == SSM_F32) launch_bwd<float, float>(a, sh, ctas, st);
-    else if (p->dtype == SSM_BF16 && p->stream_dtype == SSM_BF16) launch_bwd<__nv_bfloat16, __nv_bfloat16>(a, sh, ctas, st);
-    else if (p->dtype == SSM_BF16) launch_bwd<__nv_bfloat16, float>(a, sh, ctas, st);
-    else if (p->stream_dtype == SSM_F16) launch_bwd<__half, __half>(a, sh, ctas, st);
-    else launch_bwd<__half, float>(a, sh, ctas, st);
+    int64_t ctas;
+    if (p->dtype == SSM_F32) ctas = launch_bwd<float, float>(a, sh, st);
+    else if (p->dtype == SSM_BF16 && p->stream_dtype == SSM_BF16) ctas = launch_bwd<__nv_bfloat16, __nv_bfloat16>(a, sh, st);
+    else if (p->dtype == SSM_BF16) ctas = launch_bwd<__nv_bfloat16, float>(a, sh, st);
+    else if (p->stream_dtype == SSM_F16) ctas = launch_bwd<__half, __half>(a, sh, st);
+    else ctas = launch_bwd<__half, float>(a, sh, st);
     if (int s = check_launch("add_rmsnorm bwd")) return s;
     if (p->dweight) {
-        fold_kernel<<<(unsigned)ceil_div(a.features, 32), 256, 0, st>>>(a.part, ctas * sh.ty, a.features, p->dweight);
+        fold_kernel<<<(unsigned)ceil_div(a.features, 32), kRuns * 32, 0, st>>>(a.part, ctas * sh.ty, a.features, p->dweight);
         return check_launch("add_rmsnorm bwd: fold");
     }
     return SSM_OK;
