@@ -443,15 +443,16 @@ static int64_t esize(int dtype) { return dtype == SSM_F32 ? 4 : 2; }
 // kernels.  The forward gives a thread four vectors where the row has them: with
 // 65536 x 2560 bf16 to int8, 177 us against 189 with two and 219 with one (fewer
 // warps meet at the reduction, each with more loads on the way).  The backward,
-// which keeps three tensors' vectors, weights and sums, takes one: 505 us, 520 with
-// two and 1592 (spilled) with four.
+// which keeps three tensors' vectors, weights and sums, takes two (65536 x 2560: 425
+// us, 499 with one; four would spill), and one in rows of up to 1024, whose CTAs are
+// small enough as they are.
 struct Shape { int tx, ty, v, nv; };
 
 static Shape shape_of(int64_t F, bool vec, bool bwd) {
     const int v = vec ? 8 : 1;
     const int64_t n = ceil_div(F, v);
     int nv = 0;
-    if (vec && bwd) nv = n <= kMaxThreads ? 1 : n <= 2 * kMaxThreads ? 2 : 0;
+    if (vec && bwd) nv = n <= 128 ? 1 : n <= 2 * kMaxThreads ? 2 : 0;
     else if (vec) nv = n <= 32 ? 1 : n <= 64 ? 2 : n <= 4 * kMaxThreads ? 4 : 0;
     else nv = n <= 8 * kMaxThreads ? 8 : n <= 16 * kMaxThreads ? 16 : 0;
     if (nv == 0) return {kMaxThreads, 1, 1, 0};
