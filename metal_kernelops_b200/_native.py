@@ -313,9 +313,10 @@ def stream_here(t: torch.Tensor) -> int:
 
 
 def direct(*tensors) -> bool:
-    """Whether a call without gradients may go to the library itself instead of
-    through torch's dispatcher: the tensors are plain ones (no fake or other
-    subclass) on the current device, and nothing is being traced.  The
+    """Whether a call may go to the library itself (with a gradient: through a
+    ``torch.autograd.Function``) instead of the custom op of torch's dispatcher:
+    the tensors are plain ones (no fake or other subclass) on the current
+    device, and nothing is being traced.  The
     dispatcher's Python path costs about 15 us a call, more than the kernels
     of a decode step run for."""
     for t in tensors:

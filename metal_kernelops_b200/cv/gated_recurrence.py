@@ -97,26 +97,32 @@ def _(x, forget, z, lower, init, reset, save):
             x.new_empty(n, dtype=torch.float32))
 
 
-@torch.library.custom_op("b200ssm::gated_recurrence_bwd", mutates_args=(), device_types="cuda")
-def _bwd(dy: torch.Tensor, dfinal: Optional[torch.Tensor], x: torch.Tensor, forget: torch.Tensor,
-         z: Optional[torch.Tensor], lower: Optional[torch.Tensor], reset: Optional[torch.Tensor],
-         states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+def _backward_launch(dy, dfinal, x, forget, z, lower, reset, states):
+    """(dx, dforget, dz, dlower, dinitial), None for what the call did not have."""
     p = _params(x, forget, z, lower, None, reset, dy)
     _, ws_bytes = _sizes(p)
     dev = x.device
     f32 = dict(dtype=torch.float32, device=dev)
     dx, df = (torch.empty(x.shape, dtype=x.dtype, device=dev) for _ in range(2))
-    dz = torch.empty(x.shape if z is not None else (0,), dtype=x.dtype, device=dev)
-    dlower = torch.empty(x.shape[2] if lower is not None else 0, **f32)
+    dz = torch.empty(x.shape, dtype=x.dtype, device=dev) if z is not None else None
+    dlower = torch.empty(x.shape[2], **f32) if lower is not None else None
     dinit = torch.empty((x.shape[0], x.shape[2]), **f32)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
     p.states, p.dy, p.dfinal = states.data_ptr(), dy.data_ptr(), _ptr(dfinal)
-    p.dx, p.dforget, p.dz = dx.data_ptr(), df.data_ptr(), dz.data_ptr() if z is not None else None
-    p.dlower, p.dinitial = dlower.data_ptr() if lower is not None else None, dinit.data_ptr()
+    p.dx, p.dforget, p.dz = dx.data_ptr(), df.data_ptr(), _ptr(dz)
+    p.dlower, p.dinitial = _ptr(dlower), dinit.data_ptr()
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     p.status = nat.status_word(dev, "gated_recurrence")
     nat.check(nat.lib().ssm_gated_recurrence_bwd(p, nat.stream_here(x)), "gated_linear_recurrence backward")
     return dx, df, dz, dlower, dinit
+
+
+@torch.library.custom_op("b200ssm::gated_recurrence_bwd", mutates_args=(), device_types="cuda")
+def _bwd(dy: torch.Tensor, dfinal: Optional[torch.Tensor], x: torch.Tensor, forget: torch.Tensor,
+         z: Optional[torch.Tensor], lower: Optional[torch.Tensor], reset: Optional[torch.Tensor],
+         states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    dx, df, dz, dlower, dinit = _backward_launch(dy, dfinal, x, forget, z, lower, reset, states)
+    return (dx, df, x.new_empty(0) if dz is None else dz, dinit.new_empty(0) if dlower is None else dlower, dinit)
 
 
 @_bwd.register_fake
@@ -148,6 +154,29 @@ def _backward(ctx, dy, dfinal, dstates):
 
 
 _fwd.register_autograd(_backward, setup_context=_setup)
+
+
+class _Scan(torch.autograd.Function):
+    """The same pair of launches for plain tensors, without the dispatcher's Python path."""
+
+    @staticmethod
+    def forward(ctx, x, forget, z, lower, init, reset):
+        y, final, states = _forward(x, forget, z, lower, init, reset, True)
+        ctx.save_for_backward(x, forget, z, lower, reset, states)
+        ctx.init = init is not None
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dfinal):
+        x, forget, z, lower, reset, states = ctx.saved_tensors
+        if dy is None and dfinal is None:
+            return (None,) * 6
+        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _tokens(dy)
+        dx, df, dz, dlower, dinit = _backward_launch(dy, None if dfinal is None else dfinal.contiguous(), x, forget, z,
+                                                     lower, reset, states)
+        return dx, df, dz, dlower, dinit if ctx.init else None, None
 
 
 def _update(state, x, forget, z, lower):
@@ -222,12 +251,13 @@ def gated_linear_recurrence(x, forget, z=None, lower_bound=None, initial_state=N
     lower, init = _f32(lower_bound), _f32(initial_state)
     if reset is not None and not reset.is_contiguous():
         reset = reset.contiguous()
-    if nat.wants_grad(x, forget, z, lower, init):
-        y, final, _ = torch.ops.b200ssm.gated_recurrence_fwd(x, forget, z, lower, init, reset, True)
-    elif nat.direct(x, forget, z, lower, init, reset):
+    grad = nat.wants_grad(x, forget, z, lower, init)
+    if nat.direct(x, forget, z, lower, init, reset):
+        if grad:
+            return _Scan.apply(x, forget, z, lower, init, reset)
         y, final, _ = _forward(x, forget, z, lower, init, reset, False)
-    else:
-        y, final, _ = torch.ops.b200ssm.gated_recurrence_fwd(x, forget, z, lower, init, reset, False)
+        return y, final
+    y, final, _ = torch.ops.b200ssm.gated_recurrence_fwd(x, forget, z, lower, init, reset, grad)
     return y, final
 
 

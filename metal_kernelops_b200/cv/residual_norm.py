@@ -53,12 +53,15 @@ def _features(t):
     return t if t.is_contiguous() else _rows(t, t.shape[-1])
 
 
+def _row_stride(t):
+    return 0 if t is None or t.is_contiguous() else _stride(t)
+
+
 def _params(x, residual, weight, eps, stream=None, y=None, q=None, scale=None, rstd=None):
     features = x.shape[-1]
     code = nat.dtype_code(x.dtype)
     return nat.AddRmsNormParams(
-        x.numel() // features, features, 0 if x.is_contiguous() else _stride(x),
-        0 if residual is None or residual.is_contiguous() else _stride(residual), 0, 0, code,
+        x.numel() // features, features, _row_stride(x), _row_stride(residual), 0, 0, code,
         code if residual is None else nat.dtype_code(residual.dtype),
         0 if weight is None else nat.dtype_code(weight.dtype), eps, x.data_ptr(),
         _ptr(residual), _ptr(weight), _ptr(stream), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
@@ -134,25 +137,32 @@ def _(x):
     return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[0], dtype=torch.float32)
 
 
+def _backward_launch(dy, dstream, stream, weight, rstd, eps):
+    """(dx, dresidual in the stream's type or None where dx is it, dweight); dy, dstream and stream are rows."""
+    features = dy.shape[-1]
+    dev = dy.device
+    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+    both = stream.dtype != dy.dtype
+    dres = torch.empty(dy.shape, dtype=stream.dtype, device=dev) if both else None
+    dw = torch.empty(features, dtype=torch.float32, device=dev)
+    p = nat.AddRmsNormParams(
+        dy.numel() // features, features, _row_stride(stream), 0, _row_stride(dy), _row_stride(dstream),
+        nat.dtype_code(dy.dtype), nat.dtype_code(stream.dtype), nat.dtype_code(weight.dtype), eps)
+    need = nat._SZ()
+    nat.check(nat.lib().ssm_add_rmsnorm_sizes(p, need), "add_rmsnorm backward")
+    ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=dev)
+    p.stream, p.weight, p.rstd, p.dy, p.dx = (t.data_ptr() for t in (stream, weight, rstd, dy, dx))
+    p.dstream, p.dresidual, p.dweight = _ptr(dstream), _ptr(dres), dw.data_ptr()
+    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+    nat.check(nat.lib().ssm_add_rmsnorm_bwd(p, nat.stream_here(dy)), "add_rmsnorm backward")
+    return dx, dres, dw
+
+
 @torch.library.custom_op("b200ssm::add_rmsnorm_bwd", mutates_args=(), device_types="cuda")
 def _bwd(dy: torch.Tensor, dstream: Optional[torch.Tensor], stream: torch.Tensor, weight: torch.Tensor,
          rstd: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    rows, features = dy.shape
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    both = stream.dtype != dy.dtype                 # the stream's gradient in its own type
-    dres = torch.empty(dy.shape if both else (0,), dtype=stream.dtype, device=dy.device)
-    dw = torch.empty(features, dtype=torch.float32, device=dy.device)
-    p = nat.AddRmsNormParams(
-        rows, features, _stride(stream), 0, _stride(dy), _stride(dstream), nat.dtype_code(dy.dtype),
-        nat.dtype_code(stream.dtype), nat.dtype_code(weight.dtype), eps)
-    need = nat._SZ()
-    nat.check(nat.lib().ssm_add_rmsnorm_sizes(p, need), "add_rmsnorm backward")
-    ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=dy.device)
-    p.stream, p.weight, p.rstd, p.dy, p.dx = (t.data_ptr() for t in (stream, weight, rstd, dy, dx))
-    p.dstream, p.dresidual, p.dweight = _ptr(dstream), dres.data_ptr() if both else None, dw.data_ptr()
-    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-    nat.check(nat.lib().ssm_add_rmsnorm_bwd(p, nat.stream_of(dy)), "add_rmsnorm backward")
-    return dx, dres, dw
+    dx, dres, dw = _backward_launch(dy, dstream, stream, weight, rstd, eps)
+    return dx, _none_empty(dres, dy, stream.dtype), dw
 
 
 @_bwd.register_fake
@@ -183,6 +193,33 @@ def _backward(ctx, dy, dstream, drstd):
 
 
 _fwd.register_autograd(_backward, setup_context=_setup)
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    """The same pair of launches for plain tensors, without the dispatcher's Python path."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        rows = _features(x)
+        y, stream, rstd = _forward(rows, weight, None if residual is None else _features(residual), eps, True, x.shape)
+        ctx.save_for_backward(rows if residual is None else stream, weight, rstd)
+        ctx.eps, ctx.residual, ctx.like = eps, residual is not None, (x.shape, x.dtype)
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, stream)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dstream=None):
+        stream, weight, rstd = ctx.saved_tensors
+        if dy is None and dstream is None:
+            return None, None, None, None
+        shape, dtype = ctx.like
+        dy = torch.zeros(shape, dtype=dtype, device=stream.device) if dy is None else _features(dy)
+        dx, dres, dw = _backward_launch(dy, None if dstream is None else _features(dstream), stream, weight, rstd,
+                                        ctx.eps)
+        dx = dx.view(shape)
+        return (dx, dw if dw.dtype == weight.dtype else dw.to(weight.dtype),
+                None if not ctx.residual else dx if dres is None else dres.view(shape), None)
 
 
 def _check(name, x, weight, residual):
@@ -225,14 +262,17 @@ def add_rmsnorm(x, weight, residual=None, eps=1e-5):
     if x.numel() == 0:
         return x.new_empty(x.shape), x if residual is None else x + residual
     w = weight if weight.is_contiguous() else weight.contiguous()
-    if not nat.wants_grad(x, weight, residual) and nat.direct(x, w, residual):
+    grad = nat.wants_grad(x, weight, residual)
+    if nat.direct(x, w, residual):
+        if grad:
+            out = _AddRmsNorm.apply(x, w, residual, float(eps))
+            return (out, x) if residual is None else out
         y, stream, _ = _forward(_features(x), w, None if residual is None else _features(residual), float(eps),
                                 False, x.shape)
         return y, x if residual is None else stream
     features = x.shape[-1]
     y, stream, _ = torch.ops.b200ssm.add_rmsnorm_fwd(
-        _rows(x, features), w, None if residual is None else _rows(residual, features), float(eps),
-        nat.wants_grad(x, weight, residual))
+        _rows(x, features), w, None if residual is None else _rows(residual, features), float(eps), grad)
     return y.view(x.shape), x if residual is None else stream.view(x.shape)
 
 

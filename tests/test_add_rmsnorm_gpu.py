@@ -250,6 +250,22 @@ def test_through_the_dispatcher():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("stream", [None, BF16, F32])
+def test_gradients_through_the_dispatcher(stream):
+    """The registered op's autograd formula gives the direct call's gradients, on strided rows too."""
+    x = _make((6, 300), BF16, 1)[:, :256].requires_grad_(True)
+    res = None if stream is None else _make((6, 256), stream, 2).requires_grad_(True)
+    w = (1 + 0.1 * _make((256,), F32, 3)).requires_grad_(True)
+    leaves = [t for t in (x, w, res) if t is not None]
+    a = _cv().add_rmsnorm(x, w, res)
+    b = torch.ops.b200ssm.add_rmsnorm_fwd(x, w, res, 1e-5, True)
+    up = [_make((6, 512), BF16, 4)[:, 256:]] + ([] if res is None else [_make((6, 256), stream, 5)])
+    ga = torch.autograd.grad(a[:len(up)], leaves, up)
+    gb = torch.autograd.grad(b[:len(up)], leaves, up)
+    assert all(torch.equal(u, v) for u, v in zip(ga, gb))
+
+
+@pytest.mark.gpu
 def test_no_gradient_is_an_error():
     cv = _cv()
     x = torch.ones(2, 8, device="cuda", requires_grad=True)

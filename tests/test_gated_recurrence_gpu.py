@@ -304,6 +304,22 @@ def test_through_the_dispatcher():
 
 
 @pytest.mark.gpu
+def test_gradients_through_the_dispatcher():
+    """The registered op's autograd formula gives the direct call's gradients."""
+    t = {k: v.cuda().requires_grad_(v.is_floating_point()) for k, v in _make(2, 90, 64, BF16, True, True, True, True).items()}
+    names = [k for k in t if k != "reset"]
+    a = _cv().gated_linear_recurrence(t["x"], t["forget"], t["z"], t["lower"], t["init"], t["reset"])
+    b = torch.ops.b200ssm.gated_recurrence_fwd(t["x"], t["forget"], t["z"], t["lower"], t["init"], t["reset"], True)
+    ups = (torch.ones_like(a[0]), torch.ones_like(a[1]))
+    ga = torch.autograd.grad(a, [t[k] for k in names], ups)
+    gb = torch.autograd.grad(b[:2], [t[k] for k in names], ups)
+    assert all(torch.equal(u, v) for u, v in zip(ga, gb))
+    c = torch.ops.b200ssm.gated_recurrence_fwd(t["x"], t["forget"], None, None, None, None, True)
+    d = _cv().gated_linear_recurrence(t["x"], t["forget"])
+    assert torch.equal(torch.autograd.grad(c[0].sum(), t["forget"])[0], torch.autograd.grad(d[0].sum(), t["forget"])[0])
+
+
+@pytest.mark.gpu
 def test_update_without_gradient_is_an_error():
     s = torch.zeros(2, 8, device="cuda")
     x = torch.ones(2, 8, device="cuda", requires_grad=True)
