@@ -26,6 +26,7 @@
 // fixed order, so results are reproducible.  Rows wider than the registers of a
 // CTA hold (16384 features forward, 8192 backward) stream: a CTA reads such a row
 // twice, the second time from L1 / L2.
+#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -532,8 +533,8 @@ static int64_t most_ctas(int64_t rows, const Shape& s) {
 // As many of them as the GPU holds at once.
 template <auto kernel>
 static int64_t launch_rows(Args& a, const Shape& s, cudaStream_t st) {
-    static int room[kMaxThreads / 32 + 1];            // CTAs per SM by warps; 0: not asked yet
-    int& n = room[s.tx * s.ty / 32];
+    static std::atomic<int> room[kMaxThreads / 32 + 1];   // CTAs per SM by warps; 0: not asked yet
+    std::atomic<int>& n = room[s.tx * s.ty / 32];
     if (n == 0) {
         int k = 0;
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&k, kernel, s.tx * s.ty, 0) != cudaSuccess || k < 1) {

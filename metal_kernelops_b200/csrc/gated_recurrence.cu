@@ -36,6 +36,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <climits>
 #include <mutex>
 #include <type_traits>
@@ -711,8 +712,9 @@ static int validate(const ssm_gated_recurrence_params* p) {
     if (p == nullptr) return fail(SSM_ERR_INVALID, "gated_linear_recurrence: null params");
     if (p->batch < 0 || p->length < 0 || p->dim < 1)
         return fail(SSM_ERR_INVALID, "gated_linear_recurrence: batch, length and dim");
-    if (p->batch > 65535 || p->length > INT32_MAX || p->dim > INT32_MAX)
-        return fail(SSM_ERR_UNSUPPORTED, "gated_linear_recurrence: batch above 65535, or length or dim above 2^31 - 1");
+    if (p->batch > 65535 || p->length > INT32_MAX - 65536 || p->dim > INT32_MAX - 65536)
+        return fail(SSM_ERR_UNSUPPORTED,
+                    "gated_linear_recurrence: batch above 65535, or length or dim above 2^31 - 65537");
     if (p->dtype < SSM_F32 || p->dtype > SSM_F16) return fail(SSM_ERR_UNSUPPORTED, "gated_linear_recurrence: dtype");
     for (int64_t s : {p->x_token_stride, p->forget_token_stride, p->z_token_stride, p->dy_token_stride})
         if (s && s < p->dim) return fail(SSM_ERR_INVALID, "gated_linear_recurrence: a token stride is below dim");
@@ -802,7 +804,7 @@ static bool tma_ok(const Args& a, int dtype, bool bwd) {
 // with 2, 308 with 5; at 16 x 4096 x 5120 (1280 tiles) C = 1 is best.
 template <auto kernel>
 static int cluster_of(int64_t tiles, int64_t chunks, size_t smem) {
-    static int room[kMaxCluster + 1];              // clusters that fit at once, by size; 0: not asked yet
+    static std::atomic<int> room[kMaxCluster + 1]; // clusters that fit at once, by size; 0: not asked yet
     double best = 0.0;
     int size = 1;
     for (int c = 1; c <= kMaxCluster && c <= chunks; ++c) {

@@ -24,6 +24,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <climits>
 #include <mutex>
 
@@ -486,8 +487,9 @@ static int validate(const ssm_int8_linear_params* p) {
         return fail(SSM_ERR_INVALID, "int8_linear: tokens, in_features and out_features");
     if (p->in_features > kMaxK)
         return fail(SSM_ERR_UNSUPPORTED, "int8_linear: in_features above 131071 (the int32 sums could overflow)");
-    if (p->tokens > INT32_MAX || p->out_features > INT32_MAX)
-        return fail(SSM_ERR_UNSUPPORTED, "int8_linear: more than 2^31 - 1 tokens or out_features");
+    // tile coordinates are 32-bit, a tile's overhang included
+    if (p->tokens > INT32_MAX - 1024 || p->out_features > INT32_MAX - 1024)
+        return fail(SSM_ERR_UNSUPPORTED, "int8_linear: more than 2^31 - 1025 tokens or out_features");
     if (p->out_dtype < SSM_F32 || p->out_dtype > SSM_F16) return fail(SSM_ERR_UNSUPPORTED, "int8_linear: out_dtype");
     if ((p->x_row_stride && p->x_row_stride < p->in_features) || (p->w_row_stride && p->w_row_stride < p->in_features))
         return fail(SSM_ERR_INVALID, "int8_linear: a row stride is below in_features");
@@ -532,7 +534,7 @@ static int encode(CUtensorMap* m, const void* base, int64_t k, int64_t rows, int
 // and tensor memory say how many more share it.
 template <typename O, int NT>
 static int64_t clusters_at_once(int S, int C) {
-    static int alone[9];                             // with one CTA an SM; 0: not asked yet
+    static std::atomic<int> alone[9];                // with one CTA an SM; 0: not asked yet
     if (alone[C] == 0) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(C);
