@@ -48,7 +48,11 @@ namespace ssm {
 namespace glr {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kFwdSteps = 16, kBwdSteps = 8;         // a warp's steps of a chunk
+// A warp's steps of a chunk.  The forward holds 16 (its two factors a step and z fill
+// the 128 registers of two CTAs per SM): 1 x 4096 x 2560 bf16 with gate takes 31 us, 37
+// with 8 and three CTAs per SM, whose exchange comes twice as often.  The backward
+// holds more for a step, so 8.
+constexpr int kFwdSteps = 16, kBwdSteps = 8;
 constexpr int kMaxCluster = 8;
 constexpr int kRow = 128;                           // bytes of a step of one tensor
 
@@ -798,10 +802,10 @@ static bool tma_ok(const Args& a, int dtype, bool bwd) {
 // CTAs of a cluster.  With C of them a tile takes ceil(chunks / C) rounds, and the
 // tiles run in as many waves as the GPU's room for such clusters needs; a round of a
 // cluster costs 12 % and 6 % more per CTA than a lone CTA's (the exchange, and the
-// spread of its CTAs).  The C with the least product is taken.  Measured at 1 x 4096
-// x 5120 bf16 with gate (80 tiles, room for 296 CTAs): forward 83 us with C = 1, 67
-// with 2, 52 with 3, 60 with 4; at 2 x 16384 x 5120 (160 tiles): 437 with 1, 386
-// with 2, 308 with 5; at 16 x 4096 x 5120 (1280 tiles) C = 1 is best.
+// spread of its CTAs).  The C with the least product is taken.  Measured, forward, bf16
+// with gate, room for 296 CTAs: 1 x 4096 x 5120 (80 tiles) 59 us with C = 1, 45 with 3,
+// 51 with 4; 2 x 16384 x 5120 (160 tiles) 365 us with 1, 309 with 2, 264 with 4, 299
+// with 8; 16 x 4096 x 5120 (1280 tiles) 411 us with 1, 451 with 2.
 template <auto kernel>
 static int cluster_of(int64_t tiles, int64_t chunks, size_t smem) {
     static std::atomic<int> room[kMaxCluster + 1]; // clusters that fit at once, by size; 0: not asked yet
