@@ -306,6 +306,24 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def like(t: torch.Tensor, shape, dtype) -> torch.Tensor:
+    """A dense tensor of ``shape`` (t's, or its rows) and ``dtype`` on t's device:
+    ``empty_like`` takes half of ``torch.empty``'s 3 us."""
+    if t.shape == shape and t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return torch.empty(shape, dtype=dtype, device=t.device)
+
+
+def vector(n: int, t: torch.Tensor) -> torch.Tensor:
+    """n float32 values on t's device."""
+    return torch.empty_strided((n,), (1,), dtype=torch.float32, device=t.device)
+
+
+def matrix(m: int, n: int, dtype, t: torch.Tensor) -> torch.Tensor:
+    """A dense (m, n) tensor on t's device."""
+    return torch.empty_strided((m, n), (n, 1), dtype=dtype, device=t.device)
+
+
 def stream_here(t: torch.Tensor) -> int:
     """The current stream's handle on t's device (as :func:`stream_of`, without
     the 2 us of building a Stream object)."""

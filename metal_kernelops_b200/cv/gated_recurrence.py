@@ -70,9 +70,9 @@ def _sizes(p):
 
 def _forward(x, forget, z, lower, init, reset, save):
     p = _params(x, forget, z, lower, init, reset)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    final = torch.empty((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
-    states = torch.empty(_sizes(p)[0] // 4, dtype=torch.float32, device=x.device) if save else None
+    y = nat.like(x, x.shape, x.dtype)
+    final = nat.matrix(x.shape[0], x.shape[2], torch.float32, x)
+    states = nat.vector(_sizes(p)[0] // 4, x) if save else None
     p.y, p.final_state, p.states = y.data_ptr(), final.data_ptr(), _ptr(states)
     p.status = nat.status_word(x.device, "gated_recurrence")
     nat.check(nat.lib().ssm_gated_recurrence_fwd(p, nat.stream_here(x)), "gated_linear_recurrence")
@@ -102,16 +102,15 @@ def _backward_launch(dy, dfinal, x, forget, z, lower, reset, states):
     p = _params(x, forget, z, lower, None, reset, dy)
     _, ws_bytes = _sizes(p)
     dev = x.device
-    f32 = dict(dtype=torch.float32, device=dev)
-    dx, df = (torch.empty(x.shape, dtype=x.dtype, device=dev) for _ in range(2))
-    dz = torch.empty(x.shape, dtype=x.dtype, device=dev) if z is not None else None
-    dlower = torch.empty(x.shape[2], **f32) if lower is not None else None
-    dinit = torch.empty((x.shape[0], x.shape[2]), **f32)
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+    dx, df = nat.like(x, x.shape, x.dtype), nat.like(x, x.shape, x.dtype)
+    dz = nat.like(x, x.shape, x.dtype) if z is not None else None
+    dlower = nat.vector(x.shape[2], x) if lower is not None else None
+    dinit = nat.matrix(x.shape[0], x.shape[2], torch.float32, x)
+    ws = nat.vector(ws_bytes // 4 + 1, x)
     p.states, p.dy, p.dfinal = states.data_ptr(), dy.data_ptr(), _ptr(dfinal)
     p.dx, p.dforget, p.dz = dx.data_ptr(), df.data_ptr(), _ptr(dz)
     p.dlower, p.dinitial = _ptr(dlower), dinit.data_ptr()
-    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+    p.workspace, p.workspace_bytes = ws.data_ptr(), ws_bytes
     p.status = nat.status_word(dev, "gated_recurrence")
     nat.check(nat.lib().ssm_gated_recurrence_bwd(p, nat.stream_here(x)), "gated_linear_recurrence backward")
     return dx, df, dz, dlower, dinit
@@ -179,11 +178,23 @@ class _Scan(torch.autograd.Function):
         return dx, df, dz, dlower, dinit if ctx.init else None, None
 
 
+def _rows(t):
+    """t itself where its channels are contiguous and its rows do not overlap, else a contiguous copy."""
+    if t is None or t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
+
+
+def _row_stride(t):
+    """Elements between rows (0: dense)."""
+    return 0 if t is None or t.is_contiguous() or t.shape[0] == 1 else t.stride(0)
+
+
 def _update(state, x, forget, z, lower):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    batch, dim = x.shape
+    y = nat.matrix(batch, dim, x.dtype, x)
     p = nat.GatedRecurrenceStepParams(
-        x.shape[0], x.shape[1], *(0 if t is None or t.is_contiguous() or t.shape[0] == 1 else t.stride(0)
-                                  for t in (x, forget, z, state)),
+        batch, dim, _row_stride(x), _row_stride(forget), _row_stride(z), _row_stride(state),
         nat.dtype_code(x.dtype), 0, x.data_ptr(), forget.data_ptr(), _ptr(z), _ptr(lower), state.data_ptr(),
         y.data_ptr())
     nat.check(nat.lib().ssm_gated_recurrence_step(p, nat.stream_here(x)), "gated_linear_recurrence_update")
@@ -280,11 +291,7 @@ def gated_linear_recurrence_update(state, x, forget, z=None, lower_bound=None):
     if nat.wants_grad(state, x, forget, z, lower_bound):
         raise ValueError("gated_linear_recurrence_update has no gradient: call it under torch.no_grad()")
 
-    def rows(t):
-        ok = t is None or t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1])
-        return t if ok else t.contiguous()
-
-    x, forget, z, lower = rows(x), rows(forget), rows(z), _f32(lower_bound)
+    x, forget, z, lower = _rows(x), _rows(forget), _rows(z), _f32(lower_bound)
     if nat.direct(x, state, forget, z, lower):
         return _update(state, x, forget, z, lower)
     return torch.ops.b200ssm.gated_recurrence_update(state, x, forget, z, lower)

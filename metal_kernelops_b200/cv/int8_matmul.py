@@ -43,8 +43,9 @@ def _stride(t):
 
 def _forward(x, x_scale, weight, weight_scale, bias, out_dtype):
     features, k = weight.shape
-    dev = x.device
-    out = torch.empty((*x.shape[:-1], features), dtype=out_dtype, device=dev)
+    shape, dev = x.shape, x.device
+    out = (nat.matrix(shape[0], features, out_dtype, x) if len(shape) == 2
+           else torch.empty((*shape[:-1], features), dtype=out_dtype, device=dev))
     xp, wp, xr, wr = x.data_ptr(), weight.data_ptr(), _stride(x), _stride(weight)
     p = nat.Int8LinearParams(
         x.numel() // k, k, features, xr, wr, nat.dtype_code(out_dtype), 0, xp, x_scale.data_ptr(), wp,

@@ -67,30 +67,32 @@ def _params(x, residual, weight, eps, stream=None, y=None, q=None, scale=None, r
         _ptr(residual), _ptr(weight), _ptr(stream), _ptr(y), _ptr(q), _ptr(scale), _ptr(rstd))
 
 
+def _per_row(shape, x):
+    return nat.vector(shape[0], x) if len(shape) == 2 else torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+
+
 # The launches.  `shape` is the outputs' shape; x and residual are its rows.
 def _forward(x, weight, residual, eps, save, shape):
-    dev = x.device
-    y = torch.empty(shape, dtype=x.dtype, device=dev)
-    stream = None if residual is None else torch.empty(shape, dtype=residual.dtype, device=dev)
-    rstd = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if save else None
+    y = nat.like(x, shape, x.dtype)
+    stream = None if residual is None else nat.like(residual, shape, residual.dtype)
+    rstd = _per_row(shape, x) if save else None
     p = _params(x, residual, weight, eps, stream, y, rstd=rstd)
     nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_here(x)), "add_rmsnorm")
     return y, stream, rstd
 
 
 def _forward_int8(x, weight, residual, eps, shape):
-    dev = x.device
-    q = torch.empty(shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
-    stream = None if residual is None else torch.empty(shape, dtype=residual.dtype, device=dev)
+    q = nat.like(x, shape, torch.int8)
+    scale = _per_row(shape, x)
+    stream = None if residual is None else nat.like(residual, shape, residual.dtype)
     p = _params(x, residual, weight, eps, stream, q=q, scale=scale)
     nat.check(nat.lib().ssm_add_rmsnorm_fwd(p, nat.stream_here(x)), "add_rmsnorm_int8")
     return q, scale, stream
 
 
 def _quantize(x, shape):
-    q = torch.empty(shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    q = nat.like(x, shape, torch.int8)
+    scale = _per_row(shape, x)
     nat.check(nat.lib().ssm_quantize_int8(_params(x, None, None, 0.0, q=q, scale=scale), nat.stream_here(x)),
               "quantize_int8")
     return q, scale
@@ -140,20 +142,18 @@ def _(x):
 def _backward_launch(dy, dstream, stream, weight, rstd, eps):
     """(dx, dresidual in the stream's type or None where dx is it, dweight); dy, dstream and stream are rows."""
     features = dy.shape[-1]
-    dev = dy.device
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-    both = stream.dtype != dy.dtype
-    dres = torch.empty(dy.shape, dtype=stream.dtype, device=dev) if both else None
-    dw = torch.empty(features, dtype=torch.float32, device=dev)
+    dx = nat.like(dy, dy.shape, dy.dtype)
+    dres = nat.like(dy, dy.shape, stream.dtype) if stream.dtype != dy.dtype else None
+    dw = nat.vector(features, dy)
     p = nat.AddRmsNormParams(
         dy.numel() // features, features, _row_stride(stream), 0, _row_stride(dy), _row_stride(dstream),
         nat.dtype_code(dy.dtype), nat.dtype_code(stream.dtype), nat.dtype_code(weight.dtype), eps)
     need = nat._SZ()
     nat.check(nat.lib().ssm_add_rmsnorm_sizes(p, need), "add_rmsnorm backward")
-    ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=dev)
+    ws = nat.vector(need.value // 4 + 1, dy)
     p.stream, p.weight, p.rstd, p.dy, p.dx = (t.data_ptr() for t in (stream, weight, rstd, dy, dx))
     p.dstream, p.dresidual, p.dweight = _ptr(dstream), _ptr(dres), dw.data_ptr()
-    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
+    p.workspace, p.workspace_bytes = ws.data_ptr(), need.value
     nat.check(nat.lib().ssm_add_rmsnorm_bwd(p, nat.stream_here(dy)), "add_rmsnorm backward")
     return dx, dres, dw
 
