@@ -248,10 +248,15 @@ struct Ring {
                                          int live, int64_t c, int64_t dim) const {
         const T* p = static_cast<const T*>(tensor) + row + t * stride + c;
         const uint32_t d = tc::smem_u32(base + (s * NT + i) * kTile) + (threadIdx.x / 32 * N * 32 + (threadIdx.x & 31)) * 4;
+        if (live == N && c < dim) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const bool in = k < live && c < dim;
-            tc::cp_async4_zfill(d + k * kRow, in ? static_cast<const void*>(p + k * stride) : tensor, in ? 4u : 0u);
+            for (int k = 0; k < N; ++k, p += stride) tc::cp_async4_zfill(d + k * kRow, p, 4u);
+        } else {
+#pragma unroll 1
+            for (int k = 0; k < N; ++k, p += stride) {
+                const bool in = k < live && c < dim;
+                tc::cp_async4_zfill(d + k * kRow, in ? static_cast<const void*>(p) : tensor, in ? 4u : 0u);
+            }
         }
     }
     __device__ __forceinline__ void read(int s, int i, uint32_t* w) const {
@@ -616,8 +621,6 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 h = through<RESET>(o.A, o.H, h);
             }
         }
-        again(xw);
-        again(k);
         F hp[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
