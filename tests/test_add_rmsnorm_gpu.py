@@ -234,6 +234,27 @@ def test_empty_and_repeatable():
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last rows equal the same rows on their own."""
+    cv = _cv()
+    rows, features = (1 << 31) // 2048 + 70, 2048
+    x = torch.randn(1024, features, device="cuda", dtype=BF16).repeat(rows // 1024 + 1, 1)[:rows]
+    w = 1 + 0.1 * _make((features,), F32, 3)
+    tail = x[-300:].clone()
+    q, scale, stream = cv.add_rmsnorm_int8(x, w, x)
+    a, b, s = cv.add_rmsnorm_int8(tail, w, tail)
+    assert torch.equal(q[-300:], a) and torch.equal(scale[-300:], b) and torch.equal(stream[-300:], s)
+    del q, scale, stream
+    xs, ws = x.detach().requires_grad_(True), w.clone().requires_grad_(True)
+    y, _ = cv.add_rmsnorm(xs, ws)
+    dx, = torch.autograd.grad(y, xs, x)
+    ts = tail.requires_grad_(True)
+    z, _ = cv.add_rmsnorm(ts, ws)
+    dt, = torch.autograd.grad(z, ts, tail.detach())
+    assert torch.equal(y[-300:], z) and torch.equal(dx[-300:], dt)
+
+
+@pytest.mark.gpu
 def test_through_the_dispatcher():
     """The registered ops give what the direct calls give, and trace with fake tensors."""
     from torch._subclasses.fake_tensor import FakeTensorMode

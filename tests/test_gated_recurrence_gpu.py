@@ -285,6 +285,32 @@ def test_empty_and_repeatable():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(9, 8192, 30000), (1, 262144 + 77, 8200), (70, 4099, 7501)], ids=str)
+def test_offsets_beyond_32_bits(shape):
+    """More than 2^31 elements (by rows, by tokens, and in an odd width): the last
+    channels of the last row equal the same channels on their own."""
+    batch, length, dim = shape
+    assert batch * length * dim > 1 << 31
+    x = torch.empty(shape, device="cuda", dtype=BF16)
+    for b in range(batch):
+        x[b].normal_(generator=torch.Generator(device="cuda").manual_seed(b))
+    cut = dim - 96
+    leaf = x.requires_grad_(True)
+    y, final = _cv().gated_linear_recurrence(leaf, leaf.detach())
+    part = x.detach()[-1:, :, cut:].contiguous().requires_grad_(True)
+    yp, fp = _cv().gated_linear_recurrence(part, part.detach())
+    # other cluster sizes join other runs of steps: equal up to the limits above
+    assert bool(((y[-1:, :, cut:] - yp).float().abs() <= 2e-5 * 6 + 2 * UNIT[BF16] * yp.float().abs()).all())
+    assert bool(((final[-1:, cut:] - fp).abs() <= 2e-5 * 6).all())
+    del y, final
+    y, final = _cv().gated_linear_recurrence(leaf, leaf.detach())
+    dx, = torch.autograd.grad((y, final), leaf, (leaf.detach(), final.detach()))
+    dp, = torch.autograd.grad((yp, fp), part, (part.detach(), fp.detach()))
+    dx = dx[-1:, :, cut:]
+    assert float((dx.float() - dp.float()).norm()) <= (2e-5 + 2 * UNIT[BF16]) * float(dp.float().norm())
+
+
+@pytest.mark.gpu
 def test_through_the_dispatcher():
     cv = _cv()
     t = {k: v.cuda() for k, v in _make(2, 70, 64, BF16, True, True, True, True).items()}

@@ -123,6 +123,21 @@ def test_strided_rows_leading_axes_and_another_stream(m, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(180000, 64, 12368), (70000, 31000, 40), (200, 35000, 62000)])
+def test_offsets_beyond_32_bits(m, k, n):
+    """Results, activations or weights of more than 2^31 elements: the last rows and
+    features equal the same ones on their own."""
+    assert max(m * n, m * k, n * k) > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(-127, 128, (m, k), device="cuda", dtype=torch.int8, generator=g)
+    w = torch.randint(-127, 128, (n, k), device="cuda", dtype=torch.int8, generator=g)
+    xs, ws = torch.rand(m, device="cuda", generator=g), torch.rand(n, device="cuda", generator=g)
+    y = _cv().int8_linear(x, xs, w, ws)
+    a, b = max(0, m - 40), max(0, n - 40)
+    assert torch.equal(y[a:, b:], _cv().int8_linear(x[a:].clone(), xs[a:], w[b:].clone(), ws[b:]))
+
+
+@pytest.mark.gpu
 def test_empty_dispatcher_and_graph():
     cv = _cv()
     w, ws = _ints((24, 64), 1).cuda(), _scales(24, 2).cuda()
