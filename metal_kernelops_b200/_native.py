@@ -330,6 +330,26 @@ def stream_here(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+def same_device(name: str, index: int, named) -> None:
+    """Raise ``ValueError`` unless every tensor of ``named`` is on CUDA device ``index``
+    (negative: the first one is not on a GPU).  Called when a quick look found one that is not."""
+    for label, t in named:
+        if t is not None and (index < 0 or t.get_device() != index):
+            if not t.is_cuda:
+                raise ValueError(f"{name} runs CUDA kernels, {label} is on {t.device}")
+            raise ValueError(f"{name}: {label} is on {t.device}, {named[0][0]} is on {named[0][1].device}")
+
+
+def apart(index: int, *tensors) -> bool:
+    """Whether one of the tensors is not on CUDA device ``index``."""
+    if index < 0:
+        return True
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            return True
+    return False
+
+
 def direct(*tensors) -> bool:
     """Whether a call may go to the library itself (with a gradient: through a
     ``torch.autograd.Function``) instead of the custom op of torch's dispatcher:

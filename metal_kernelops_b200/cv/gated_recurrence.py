@@ -227,12 +227,9 @@ def _check(name, x, forget, z, lower, state, reset, axes):
     if reset is not None and (reset.shape != shape[:2] or reset.dtype not in (torch.bool, torch.uint8)):
         raise ValueError(f"reset must be bool {tuple(shape[:2])}, got {tuple(reset.shape)}, {reset.dtype}")
     index = x.get_device()                          # negative off the GPU
-    for label, t in (("x", x), ("forget", forget), ("z", z), ("lower_bound", lower), ("the state", state),
-                     ("reset", reset)):
-        if t is not None and (index < 0 or t.get_device() != index):
-            if not t.is_cuda:
-                raise ValueError(f"{name} runs CUDA kernels, {label} is on {t.device}")
-            raise ValueError(f"{name}: {label} is on {t.device}, x is on {x.device}")
+    if nat.apart(index, forget, z, lower, state, reset):
+        nat.same_device(name, index, (("x", x), ("forget", forget), ("z", z), ("lower_bound", lower),
+                                      ("the state", state), ("reset", reset)))
     if x.dtype not in _DTYPES:
         raise ValueError(f"{name} computes float32/bfloat16/float16, x is {x.dtype}")
 

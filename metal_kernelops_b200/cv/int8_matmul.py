@@ -100,11 +100,9 @@ def int8_linear(x, x_scale, weight, weight_scale, bias=None, out_dtype=torch.bfl
     if out_dtype not in _DTYPES:
         raise ValueError(f"int8_linear: out_dtype is float32/bfloat16/float16, got {out_dtype}")
     index = x.get_device()                          # negative off the GPU
-    for label, t in (("x", x), ("x_scale", x_scale), ("weight", weight), ("weight_scale", weight_scale), ("bias", bias)):
-        if t is not None and (index < 0 or t.get_device() != index):
-            if not t.is_cuda:
-                raise ValueError(f"int8_linear runs CUDA kernels, {label} is on {t.device}")
-            raise ValueError(f"int8_linear: {label} is on {t.device}, x is on {x.device}")
+    if nat.apart(index, x_scale, weight, weight_scale, bias):
+        nat.same_device("int8_linear", index, (("x", x), ("x_scale", x_scale), ("weight", weight),
+                                               ("weight_scale", weight_scale), ("bias", bias)))
     if nat.wants_grad(x_scale, weight_scale, bias):
         raise ValueError("int8_linear has no gradient: call it under torch.no_grad()")
     if 0 in shape:

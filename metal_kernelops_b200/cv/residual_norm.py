@@ -231,15 +231,11 @@ def _check(name, x, weight, residual):
     if residual is not None and residual.shape != shape:
         raise ValueError(f"residual must match x {tuple(shape)}, got {tuple(residual.shape)}")
     index = x.get_device()                          # negative off the GPU
-    for label, t in (("x", x), ("weight", weight), ("residual", residual)):
-        if t is None:
-            continue
-        if index < 0 or t.get_device() != index:
-            if not t.is_cuda:
-                raise ValueError(f"{name} runs CUDA kernels, {label} is on {t.device}")
-            raise ValueError(f"{name}: {label} is on {t.device}, x is on {x.device}")
-        if t.dtype not in _DTYPES:
-            raise ValueError(f"{name} computes float32/bfloat16/float16, {label} is {t.dtype}")
+    if nat.apart(index, weight, residual):
+        nat.same_device(name, index, (("x", x), ("weight", weight), ("residual", residual)))
+    if x.dtype not in _DTYPES or (weight is not None and weight.dtype not in _DTYPES):
+        raise ValueError(f"{name} computes float32/bfloat16/float16, x is {x.dtype}"
+                         + ("" if weight is None else f", weight {weight.dtype}"))
     if residual is not None and residual.dtype is not x.dtype and residual.dtype is not torch.float32:
         raise ValueError(f"{name}: the residual stream is {x.dtype} or float32, got {residual.dtype}")
 
