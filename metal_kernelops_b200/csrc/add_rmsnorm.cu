@@ -136,33 +136,43 @@ __device__ __forceinline__ SumMax row_reduce(SumMax v, int warps, SumMax* red) {
     return v;
 }
 
-// The int8 step's factors from max|v| of a row (as bits): v * inv rounds to q,
-// and q * scale1 stands for v.
-struct Quant { float inv, scale1; };
+// The int8 step.  q = rint(v / scale) = rint(127 v / max|v|): the quotient is formed
+// from 127 v, which is exact for 16-bit data, and is correctly rounded, so that a v
+// that lies exactly between two steps (16-bit data often do) is seen as such and goes
+// to the even one.  A product with a rounded 127 / max misses those: 2e-5 of the
+// values then differ from the definition in 64 bits, 7e-7 (fp16) so.
+// The division: with y the rounded reciprocal of the divisor b, t = n y and
+// t + (n - t b) y in fused steps is the rounded quotient (Markstein, IBM J. Res. Dev.
+// 34, 1990).  n and b carry a factor of 1 / 128, so that 127 v cannot overflow.  It
+// costs 3 % (65536 x 2560 bf16 to int8: 176 -> 182 us, HBM-bound).
+struct Quant { float b, y, scale; };             // y = 0: the row's q are zeros; q * scale stands for v
 __device__ __forceinline__ Quant quant_of(uint32_t mx) {
     const float m = __uint_as_float(mx);
-    if (mx >= 0x7f800000u) return {0.0f, __uint_as_float(0x7fc00000u)};
-    if (m < kTiny) return {0.0f, 0.0f};
-    return {127.0f / m, m / 127.0f};
+    if (mx >= 0x7f800000u) return {0.0f, 0.0f, __uint_as_float(0x7fc00000u)};
+    if (m < kTiny) return {0.0f, 0.0f, 0.0f};
+    const float b = m * 0.0078125f;
+    return {b, 1.0f / b, m / 127.0f};
 }
-// rint(v * inv) in the low byte: adding 1.5 * 2^23 leaves the rounded integer
-// (to nearest, ties to even) in the low bits of the sum.
-__device__ __forceinline__ uint32_t q_bits(float v, float inv) {
-    return __float_as_uint(fmaf(v, inv, 12582912.0f));
+// Two q in the low bytes: adding 1.5 * 2^23 leaves the rounded integer (to nearest,
+// ties to even) in the low bits of the sum.
+__device__ __forceinline__ float2 q_bits(float2 v, const Quant& s) {
+    const float2 n = mul2(v, f2(0.9921875f)), t = mul2(n, f2(s.y));
+    return add2(fma2(fma2(t, f2(-s.b), n), f2(s.y), t), f2(12582912.0f));
 }
-// A row that is not finite has inv = 0 and must store zeros, also where v is
+// A row that is not finite has y = 0 and must store zeros, also where v is
 // infinite or NaN.
-__device__ __forceinline__ uint32_t pack4(const float* v, float inv) {
-    const uint32_t lo = __byte_perm(q_bits(v[0], inv), q_bits(v[1], inv), 0x0040);
-    const uint32_t hi = __byte_perm(q_bits(v[2], inv), q_bits(v[3], inv), 0x0040);
-    return inv != 0.0f ? __byte_perm(lo, hi, 0x5410) : 0u;
+__device__ __forceinline__ uint32_t pack4(const float* v, const Quant& s) {
+    const float2 a = q_bits(make_float2(v[0], v[1]), s), b = q_bits(make_float2(v[2], v[3]), s);
+    const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+    return s.y != 0.0f ? __byte_perm(lo, hi, 0x5410) : 0u;
 }
 
 // V int8 values of a row at q.
 template <int V>
-__device__ __forceinline__ void st_q(int8_t* q, const float* v, float inv) {
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(q) = make_uint2(pack4(v, inv), pack4(v + 4, inv));
-    else *q = inv != 0.0f ? (int8_t)(q_bits(v[0], inv) & 0xffu) : (int8_t)0;
+__device__ __forceinline__ void st_q(int8_t* q, const float* v, const Quant& s) {
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(q) = make_uint2(pack4(v, s), pack4(v + 4, s));
+    else *q = s.y != 0.0f ? (int8_t)(__float_as_uint(q_bits(f2(v[0]), s).x) & 0xffu) : (int8_t)0;
 }
 
 // x (+ residual) -> s, and s stored; the V values of s.
@@ -244,12 +254,12 @@ fwd_kernel(const Args a) {
         }
     } else {
         const Quant qt = quant_of(sm.mx);
-        if (threadIdx.x == 0) a.scale[row] = qt.scale1 * r;
+        if (threadIdx.x == 0) a.scale[row] = qt.scale * r;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
             if (e < F)
-                st_q<V>(a.q + row * F + e, v[k], qt.inv);
+                st_q<V>(a.q + row * F + e, v[k], qt);
         }
     }
 }
@@ -281,14 +291,14 @@ fwd_stream_kernel(const Args a) {
     const float r = MODE == kInt8 ? 1.0f : 1.0f / sqrtf(fmaf(sm.sum, a.inv_f, a.eps));
     const Quant qt = quant_of(sm.mx);
     if (threadIdx.x == 0) {
-        if (MODE != kNorm) a.scale[row] = qt.scale1 * r;
+        if (MODE != kNorm) a.scale[row] = qt.scale * r;
         else if (a.rstd != nullptr) a.rstd[row] = r;
     }
     for (int64_t e = threadIdx.x; e < F; e += blockDim.x) {
         float v = MODE == kInt8 ? ldf(x + e) : value(e);
         if (MODE != kInt8) v *= ld_any(a.w, e, a.weight_dtype);
         if (MODE == kNorm) stf(static_cast<T*>(a.y) + row * F + e, v * r);
-        else st_q<1>(a.q + row * F + e, &v, qt.inv);
+        else st_q<1>(a.q + row * F + e, &v, qt);
     }
 }
 
@@ -442,8 +452,9 @@ static int64_t esize(int dtype) { return dtype == SSM_F32 ? 4 : 2; }
 // v elements a vector (8, or 1 where width or alignment does not allow 8), nv
 // vectors a thread, tx threads a row, ty rows a CTA; nv = 0: the streaming
 // kernels.  The forward gives a thread four vectors where the row has them: with
-// 65536 x 2560 bf16 to int8, 177 us against 189 with two and 219 with one (fewer
-// warps meet at the reduction, each with more loads on the way).  The backward,
+// 65536 x 2560 bf16 to int8 (with the plain product for q), 177 us against 189 with
+// two and 219 with one: fewer warps meet at the reduction, each with more loads on
+// the way.  The backward,
 // which keeps three tensors' vectors, weights and sums, takes two (65536 x 2560: 425
 // us, 499 with one; four would spill), and one in rows of up to 1024, whose CTAs are
 // small enough as they are.

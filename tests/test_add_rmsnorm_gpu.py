@@ -106,6 +106,39 @@ def test_quantize(case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_values_between_two_steps_go_to_the_even_one(dtype):
+    """16-bit rows whose values are exact halves of a step for many largest values
+    (127 x is exact there, in float32 it rounds): q is 127 x / max in exact rational
+    arithmetic, rounded to nearest, ties to even."""
+    g = torch.Generator().manual_seed(3)
+    m = torch.randint(1, 256, (400, 1), generator=g).double() * 2.0 ** torch.randint(-6, 6, (400, 1), generator=g)
+    n = torch.randint(-127, 127, (400, 200), generator=g).double() + 0.5
+    x = (n * m / 127).to(dtype)                      # halves where this is exact, near them elsewhere
+    x[:, ::2] = (torch.randint(-64, 64, (400, 100), generator=g).double() * m / 128).to(dtype)[:, :100]
+    x[:, 0] = m[:, 0].to(dtype)
+    x = x.clamp(-m, m).to(dtype)
+    q, _ = _cv().quantize_int8(x.cuda())
+    num, den = (x.double() * 127 * 2 ** 34).round().long(), (m * 2 ** 34).round().long()
+    assert bool((num.double() == x.double() * 127 * 2 ** 34).all())
+    low = torch.div(2 * num + den, 2 * den, rounding_mode="floor")       # floor(num / den + 1/2)
+    tie = (2 * num + den) % (2 * den) == 0
+    want = torch.where(tie & (low % 2 != 0), low - 1, low)
+    assert torch.equal(q.long().cpu(), want) and int(tie.sum()) > 100
+
+
+@pytest.mark.gpu
+def test_largest_and_smallest_rows():
+    """Rows near the ends of float32's range keep their ratios."""
+    x = torch.linspace(-1, 1, 255).repeat(3, 1)
+    big = x * torch.tensor([[3.4e38], [1.0], [2.0 ** -99]])
+    q, scale = _cv().quantize_int8(big.cuda())
+    assert torch.equal(q[0], q[1]) and torch.equal(q[2], q[1])
+    assert torch.equal(q[1].cpu(), torch.round(x[1].double() * 127).to(torch.int8))
+    assert bool(scale.isfinite().all()) and bool((scale > 0).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("case", CASES, ids=str)
 @pytest.mark.parametrize("up", ["y", "stream", "both"])
 def test_gradients(case, up):
