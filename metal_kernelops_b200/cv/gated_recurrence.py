@@ -83,7 +83,8 @@ def _forward(x, forget, z, lower, init, reset, save):
 def _fwd(x: torch.Tensor, forget: torch.Tensor, z: Optional[torch.Tensor], lower: Optional[torch.Tensor],
          init: Optional[torch.Tensor], reset: Optional[torch.Tensor],
          save: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    y, final, states = _forward(x, forget, z, lower, init, reset, save)
+    with torch.cuda.device_of(x):
+        y, final, states = _forward(x, forget, z, lower, init, reset, save)
     return y, final, final.new_empty(0) if states is None else states
 
 
@@ -120,7 +121,8 @@ def _backward_launch(dy, dfinal, x, forget, z, lower, reset, states):
 def _bwd(dy: torch.Tensor, dfinal: Optional[torch.Tensor], x: torch.Tensor, forget: torch.Tensor,
          z: Optional[torch.Tensor], lower: Optional[torch.Tensor], reset: Optional[torch.Tensor],
          states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    dx, df, dz, dlower, dinit = _backward_launch(dy, dfinal, x, forget, z, lower, reset, states)
+    with torch.cuda.device_of(x):
+        dx, df, dz, dlower, dinit = _backward_launch(dy, dfinal, x, forget, z, lower, reset, states)
     return (dx, df, x.new_empty(0) if dz is None else dz, dinit.new_empty(0) if dlower is None else dlower, dinit)
 
 
@@ -204,7 +206,8 @@ def _update(state, x, forget, z, lower):
 @torch.library.custom_op("b200ssm::gated_recurrence_update", mutates_args=("state",), device_types="cuda")
 def _step(state: torch.Tensor, x: torch.Tensor, forget: torch.Tensor, z: Optional[torch.Tensor],
           lower: Optional[torch.Tensor]) -> torch.Tensor:
-    return _update(state, x, forget, z, lower)
+    with torch.cuda.device_of(x):
+        return _update(state, x, forget, z, lower)
 
 
 @_step.register_fake

@@ -63,7 +63,8 @@ def _forward(x, x_scale, weight, weight_scale, bias, out_dtype):
 @torch.library.custom_op("b200ssm::int8_linear", mutates_args=(), device_types="cuda")
 def _op(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
         bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
-    return _forward(x, x_scale, weight, weight_scale, bias, out_dtype)
+    with torch.cuda.device_of(x):
+        return _forward(x, x_scale, weight, weight_scale, bias, out_dtype)
 
 
 @_op.register_fake

@@ -106,7 +106,8 @@ def _none_empty(t, like, dtype):
 @torch.library.custom_op("b200ssm::add_rmsnorm_fwd", mutates_args=(), device_types="cuda")
 def _fwd(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor], eps: float,
          save: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    y, stream, rstd = _forward(x, weight, residual, eps, save, x.shape)
+    with torch.cuda.device_of(x):
+        y, stream, rstd = _forward(x, weight, residual, eps, save, x.shape)
     return y, _none_empty(stream, x, x.dtype), _none_empty(rstd, x, torch.float32)
 
 
@@ -119,7 +120,8 @@ def _(x, weight, residual, eps, save):
 @torch.library.custom_op("b200ssm::add_rmsnorm_int8", mutates_args=(), device_types="cuda")
 def _int8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor],
           eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    q, scale, stream = _forward_int8(x, weight, residual, eps, x.shape)
+    with torch.cuda.device_of(x):
+        q, scale, stream = _forward_int8(x, weight, residual, eps, x.shape)
     return q, scale, _none_empty(stream, x, x.dtype)
 
 
@@ -131,7 +133,8 @@ def _(x, weight, residual, eps):
 
 @torch.library.custom_op("b200ssm::quantize_int8", mutates_args=(), device_types="cuda")
 def _quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return _quantize(x, x.shape)
+    with torch.cuda.device_of(x):
+        return _quantize(x, x.shape)
 
 
 @_quant.register_fake
@@ -161,7 +164,8 @@ def _backward_launch(dy, dstream, stream, weight, rstd, eps):
 @torch.library.custom_op("b200ssm::add_rmsnorm_bwd", mutates_args=(), device_types="cuda")
 def _bwd(dy: torch.Tensor, dstream: Optional[torch.Tensor], stream: torch.Tensor, weight: torch.Tensor,
          rstd: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    dx, dres, dw = _backward_launch(dy, dstream, stream, weight, rstd, eps)
+    with torch.cuda.device_of(dy):
+        dx, dres, dw = _backward_launch(dy, dstream, stream, weight, rstd, eps)
     return dx, _none_empty(dres, dy, stream.dtype), dw
 
 
