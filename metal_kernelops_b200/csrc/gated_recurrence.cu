@@ -12,7 +12,7 @@
 // that gates near one (long memory) keep their full relative precision.
 // Backward, with dh_t the gradient of h_t and a_t taken as 0 at a reset:
 //     dh_t = dy_t silu(z_t) + a_{t+1} dh_{t+1}   (+ dfinal at the last step)
-//     dx = g dh,  dg = dh (x - h'),  dforget = -dg g (1 - k),  dlower = -sum dg k
+//     dx = g dh,  dg = dh (x - h'),  dforget = -dg g (1 - k),  dlower = -sum dg k,  1 - k = k e^forget
 //     dz = dy h silu'(z),  dinitial = a_0 dh_0
 //
 // Both directions are scans of affine maps: a run of steps takes the state S to
@@ -106,6 +106,24 @@ __device__ __forceinline__ float2 sigmoid_neg(float2 v) {
     const float2 m = mul2(v, f2(kLog2e));
     const float2 d = add2(f2(1.0f), make_float2(exp2_mufu(m.x), exp2_mufu(m.y)));
     return make_float2(rcp_mufu(d.x), rcp_mufu(d.y));
+}
+// The same in two halves, for the backward: e^v, and k = 1 / (1 + e^v) from it.  1 - k
+// is then e^v k with the digits that k near 1 has lost; where e^v overflowed (infinity
+// times the 0 that k became) it is 1, which the minimum returns for a NaN.
+__device__ __forceinline__ float exp_of(float v) { return exp2_mufu(v * kLog2e); }
+__device__ __forceinline__ float2 exp_of(float2 v) {
+    const float2 m = mul2(v, f2(kLog2e));
+    return make_float2(exp2_mufu(m.x), exp2_mufu(m.y));
+}
+__device__ __forceinline__ float gate_of(float e) { return rcp_mufu(1.0f + e); }
+__device__ __forceinline__ float2 gate_of(float2 e) {
+    const float2 d = add2(f2(1.0f), e);
+    return make_float2(rcp_mufu(d.x), rcp_mufu(d.y));
+}
+__device__ __forceinline__ float complement(float e, float k) { return fminf(e * k, 1.0f); }
+__device__ __forceinline__ float2 complement(float2 e, float2 k) {
+    const float2 c = mul2(e, k);
+    return make_float2(fminf(c.x, 1.0f), fminf(c.y, 1.0f));
 }
 // 1 / (1 + e^-v)
 __device__ __forceinline__ float sigmoid_pos(float v) { return rcp_mufu(1.0f + exp2_mufu(v * -kLog2e)); }
@@ -534,7 +552,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         const int64_t chunk = (rounds - 1 - turn) * C + rank, t = chunk * kChunk + warp * N;
         const int live = (int)max64(0, min64(N, a.length - t));
         uint32_t xw[N], zw[N], dw[N];
-        F k[N], h;
+        F ev[N], h;                       // e^forget
         const uint32_t rs = RESET ? reset_mask<N>(a.reset, b * a.length, t, a.length) : 0u;
         ld_chan(chunk < a.chunks ? a.states + (b * a.saved + chunk) * a.dim : nullptr, c, a.dim, 0.0f, h);
         {
@@ -561,14 +579,14 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 for (int i = 0; i < N; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
             }
 #pragma unroll
-            for (int i = 0; i < N; ++i) k[i] = sigmoid_neg(unpack<T>(fw[i]));
+            for (int i = 0; i < N; ++i) ev[i] = exp_of(unpack<T>(fw[i]));
         }
         Map<F> m{one, zero};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const F av = fm(nspan, k[i], one);
+            const F k = gate_of(ev[i]), av = fm(nspan, k, one);
             if (RESET && (rs >> i & 1u)) m = {zero, zero};
-            m.H = fm(av, m.H, mu(mu(span, k[i]), unpack<T>(xw[i])));
+            m.H = fm(av, m.H, mu(mu(span, k), unpack<T>(xw[i])));
             m.A = mu(m.A, av);
         }
         F d = zero;
@@ -579,7 +597,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                 const F z = unpack<T>(zw[i]);
                 e = mu(e, mu(z, sigmoid_pos(z)));
             }
-            d = mu(ad(d, e), fm(nspan, k[i], one));
+            d = mu(ad(d, e), fm(nspan, gate_of(ev[i]), one));
             if (RESET && (rs >> i & 1u)) d = zero;
         }
         auto& mw = maps[turn & 1];
@@ -624,12 +642,13 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         F hp[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (RESET && (rs >> i & 1u)) h = zero;
             hp[i] = h;
-            h = fm(fm(nspan, k[i], one), h, mu(mu(span, k[i]), unpack<T>(xw[i])));
+            if (RESET && (rs >> i & 1u)) h = zero;
+            const F k = gate_of(ev[i]);
+            h = fm(fm(nspan, k, one), h, mu(mu(span, k), unpack<T>(xw[i])));
         }
         again(xw);
-        again(k);
+        again(ev);
         again(dw);
         if (GATE) again(zw);
         const int64_t at = (b * a.length + t + N - 1) * a.dim + c;
@@ -638,27 +657,28 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         F dl = zero;
 #pragma unroll
         for (int i = N - 1; i >= 0; --i) {
-            const F g = mu(span, k[i]), av = fm(nspan, k[i], one), x = unpack<T>(xw[i]), dy = unpack<T>(dw[i]);
+            const F k = gate_of(ev[i]), x = unpack<T>(xw[i]), dy = unpack<T>(dw[i]);
             F e = dy;
             if (GATE) {
                 const F z = unpack<T>(zw[i]), s = sigmoid_pos(z), zs = mu(z, s);
                 e = mu(dy, zs);
                 // silu'(z) = s + z s (1 - s)
                 const F ds = fm(zs, sub(one, s), s);
-                dz.put(i, mu(mu(dy, fm(av, hp[i], mu(g, x))), ds));
+                dz.put(i, mu(mu(dy, h), ds));
                 dz.move(-a.dim);
             }
             d = ad(d, e);                          // dh of step i
-            const F dg = mu(d, sub(x, hp[i]));
-            dx.put(i, mu(g, d));
+            h = hp[i];                             // what step i - 1 left
+            const F gd = mu(mu(span, k), d), before = RESET && (rs >> i & 1u) ? zero : h;
+            const F back = sub(before, x);         // -dg = dh (h' - x)
+            dx.put(i, gd);
             dx.move(-a.dim);
-            df.put(i, mu(mu(dg, g), sub(k[i], one)));
+            df.put(i, mu(mu(gd, back), complement(ev[i], k)));
             df.move(-a.dim);
-            dl = fm(dg, k[i], dl);
-            d = mu(d, av);
-            if (RESET && (rs >> i & 1u)) d = zero;
+            dl = fm(mu(d, back), k, dl);
+            d = RESET && (rs >> i & 1u) ? zero : sub(d, gd);
         }
-        dlower = sub(dlower, dl);
+        dlower = ad(dlower, dl);
     }
     if (C > 1) cluster.sync();                          // nothing is on its way to a CTA that ends
     if (warp == 0 && rank == 0 && a.dinit != nullptr) st_chan(a.dinit + b * a.dim, c, a.dim, D);
