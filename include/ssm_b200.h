@@ -492,6 +492,8 @@ int ssm_gated_rmsnorm_bwd(const ssm_gated_rmsnorm_params* p, void* stream);
  * residual may be NULL; stream is then not written.  rstd may be NULL in the
  * forward.  A row that holds a NaN or an infinity gets scale = NaN and q = 0; a
  * row whose largest |weight s| is below 2^-100 gets scale = 0 and q = 0.
+ * A finite row is right up to the largest values of its type where every weight s
+ * is finite in fp32 (one that is not counts as infinite).
  * The backward reads `stream` (x itself without a residual, with stream_dtype =
  * dtype and x_row_stride its row stride) and rstd; dstream and dresidual may be
  * NULL, dweight too (not written).  It takes a workspace of

@@ -13,7 +13,8 @@
 // non-negative floats their order is the values' order, with infinities and then
 // NaN above every finite value, so a row that holds one is recognised; its scale
 // is NaN and its q zero, and what reads it is NaN rather than silently finite.
-// Rows whose largest |y| (before the factor rstd) is below 2^-100 count as zero.
+// Rows whose largest |y| (before the factor rstd) is below 2^-100 count as zero.  A finite row
+// whose squares do not fit fp32 is added up a second time, scaled down; |w s| has to fit.
 // Backward, with xh = s rstd and c = mean(w dy xh):
 //     d  = rstd (w dy - xh c) + dstream,   dx = dresidual = d,   dw = sum_rows dy xh
 //
@@ -192,6 +193,31 @@ __device__ __forceinline__ void sum_store(const Args& a, int64_t row, int64_t e,
     }
 }
 
+// rstd of a row whose sum of squares left fp32's range (an |s| above 1.8e19 does that): every
+// warp of the row adds the squares of 2^-84 s, from s as it is stored.  What overflowed adds up
+// to at least 2^-40 then, and 2^31 of the largest squares to 2^119.  A row that holds an infinity
+// gets 0, as 1 / sqrt(infinity) is.  Called behind the reduction's barrier, so the other
+// warps' stores are seen; a row of a single warp has to order its lanes' itself.
+template <typename T, typename TS>
+__device__ __forceinline__ float rstd_of_large(const Args& a, int64_t row) {
+    constexpr float kDown = 5.169878828456423e-26f;     // 2^-84
+    __syncwarp();
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    const TS* s = static_cast<const TS*>(a.stream) + row * a.features;
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int64_t e = threadIdx.x & 31; e < a.features; e += 32) {
+        const float v = (a.res != nullptr ? ldf(s + e) : ldf(x + e)) * kDown;
+        sum = fmaf(v, v, sum);
+    }
+    return kDown / sqrtf(fmaf(sum_low_lanes<32>(sum), a.inv_f, a.eps * kDown * kDown));
+}
+template <typename T, typename TS>
+__device__ __forceinline__ float rstd_of(const Args& a, int64_t row, float sum) {
+    if (sum == __int_as_float(0x7f800000)) return rstd_of_large<T, TS>(a, row);
+    return 1.0f / sqrtf(fmaf(sum, a.inv_f, a.eps));
+}
+
 enum Mode { kNorm, kNormInt8, kInt8 };    // y, q and scale, q and scale of x itself
 
 template <typename T, typename TS, int V, int NV, int MODE>
@@ -238,7 +264,7 @@ fwd_kernel(const Args a) {
     }
     sm = row_reduce(sm, warps, red);
     if (!live) return;
-    const float r = MODE == kInt8 ? 1.0f : 1.0f / sqrtf(fmaf(sm.sum, a.inv_f, a.eps));
+    const float r = MODE == kInt8 ? 1.0f : rstd_of<T, TS>(a, row, sm.sum);
     if (MODE == kNorm) {
         if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = r;
 #pragma unroll
@@ -288,7 +314,7 @@ fwd_stream_kernel(const Args a) {
         if (MODE != kNorm) sm.mx = max(sm.mx, abs_bits(v));
     }
     sm = row_reduce(sm, blockDim.x >> 5, red);
-    const float r = MODE == kInt8 ? 1.0f : 1.0f / sqrtf(fmaf(sm.sum, a.inv_f, a.eps));
+    const float r = MODE == kInt8 ? 1.0f : rstd_of<T, TS>(a, row, sm.sum);
     const Quant qt = quant_of(sm.mx);
     if (threadIdx.x == 0) {
         if (MODE != kNorm) a.scale[row] = qt.scale * r;

@@ -19,7 +19,8 @@ bfloat16 or float16 with any leading shape, weight any of the three.
   scale per output channel).
 
 A row that holds a NaN or an infinity has scale NaN (what reads it is NaN, not
-silently finite); a row of zeros has scale 0.  The int8 functions have no
+silently finite); a row of zeros has scale 0.  Finite rows may be as large as their type allows, as
+long as ``weight * stream`` stays inside float32: an element past it counts as infinite.  The int8 functions have no
 gradient and say so when one is asked for.  The reference has no counterpart.
 CUDA tensors only; kernels in ``csrc/add_rmsnorm.cu``.
 """
