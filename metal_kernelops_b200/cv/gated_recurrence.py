@@ -17,6 +17,10 @@ float16; the state is float32 throughout.
 * :func:`gated_linear_recurrence_update` takes one token per row and updates
   the state in place.
 
+Gates are computed in float32 from approximate exponentials: ``g`` errs by up to
+``(1.25 |forget| + 10) / 2**24`` of itself.  Steady gates near one keep their memory over long
+rows: 65536 steps with ``forget`` of 8 to 12 stay within 4e-5 of the definition.
+
 The reference has no counterpart.  CUDA tensors only; kernels in
 ``csrc/gated_recurrence.cu``.
 """

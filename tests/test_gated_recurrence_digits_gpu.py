@@ -175,3 +175,138 @@ def test_gradient_of_a_wide_open_gate():
     want = -1.5 * torch.sigmoid(-d) * torch.sigmoid(d)
     eta = (1.25 * d.abs() + 10) * 2.0 ** -24
     assert bool(((got.double().cpu() - want).abs() <= (2 * eta + 2.0 ** -22) * want.abs()).all())
+
+
+# ------------------------------------------------------------- long memories --
+# Gates that write g of a step, from 3.4e-5 to 6e-6, over 65536 steps.  A gate's own error moves the
+# result by at most 2 eta <= 3e-6 of the largest magnitude M that entered, the roundings inside a
+# chunk 2e-6.  The state passes from chunk to chunk 512 times at most (1024 in the backward), each
+# time with a rounding of 2^-25: 3.1e-5 if all went one way.  Together below 4e-5 of M.
+LONG = [(8.0, 0.9), (10.0, 0.0), (12.0, 0.0), (-3.0, 0.9999)]
+
+
+def _steady(value, low, length):
+    """(g, a^t for t = 1 ... length) of a steady gate, float64."""
+    k = torch.sigmoid(torch.tensor(-value, dtype=torch.float64))
+    g = (1 - torch.tensor(low).double()) * k
+    return g, torch.exp(torch.arange(1, length + 1, dtype=torch.float64) * torch.log1p(-g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 70, 33, 20480], ids=lambda d: f"dim{d}")
+@pytest.mark.parametrize("value,low", LONG)
+def test_steady_gates_over_a_long_row(value, low, dim, dtype):
+    """Constant inputs: h_t = x + a^t (h_0 - x), by TMA, by word copies and by direct loads, with clusters
+    and without."""
+    length = 65536 if dim < 1000 else 8192
+    _, decay = _steady(value, low, length)
+    x = torch.full((1, 1, 1), 0.5, device="cuda", dtype=dtype).expand(1, length, dim).contiguous()
+    f = torch.full_like(x, value)
+    init, lower = torch.full((1, dim), 2.0, device="cuda"), torch.full((dim,), low, device="cuda")
+    y, final = _cv().gated_linear_recurrence(x, f, None, lower, init)
+    want = 0.5 + decay * 1.5
+    assert bool(((final.double().cpu() - want[-1]).abs() <= 4e-5 * 2).all()), float((final.double().cpu() - want[-1]).abs().max())
+    for c in (0, dim - 1):
+        err = (y[0, :, c].double().cpu() - want).abs()
+        assert bool((err <= 4e-5 * 2 + (UNIT[dtype] if dtype != F32 else 0) * want).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 33, 20480], ids=lambda d: f"dim{d}")
+@pytest.mark.parametrize("value,low", LONG)
+def test_gradients_of_steady_gates_over_a_long_row(value, low, dim):
+    """dfinal = 1, dy = 0: dx_t = g a^(T - t), dinitial = a^T."""
+    length = 65536 if dim < 1000 else 8192
+    g, decay = _steady(value, low, length)
+    x = torch.zeros(1, length, dim, device="cuda", requires_grad=True)
+    f = torch.full((1, length, dim), value, device="cuda")
+    init = torch.zeros(1, dim, device="cuda", requires_grad=True)
+    _, final = _cv().gated_linear_recurrence(x, f, None, torch.full((dim,), low, device="cuda"), init)
+    dx, dinit = torch.autograd.grad(final.sum(), (x, init))
+    assert bool(((dinit.double().cpu() - decay[-1]).abs() <= 4e-5).all())
+    want = g * torch.cat([decay.flip(0)[1:], torch.ones(1, dtype=torch.float64)])
+    for c in (0, dim - 1):
+        assert bool(((dx[0, :, c].double().cpu() - want).abs() <= 4.5e-5 * g).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value,low", LONG)
+def test_steps_with_steady_gates(value, low):
+    """65536 single tokens: every step rounds the state once, 2^-25 of it; roundings of a state that
+    moves differ in sign (their sum grows as the root of the count, 1e-5 at 3 sigma), and near the end value
+    they cannot exceed 2^-25 / g of it, whichever way they go: 9e-4 at g = 3.4e-5.  Both are far
+    below what a one-sided error would add up to, 2e-3; the limit is 1e-4 of the largest value."""
+    length = 65536
+    _, decay = _steady(value, low, length)
+    x = torch.full((3, 64), 0.5, device="cuda")
+    f, lower = torch.full_like(x, value), torch.full((64,), low, device="cuda")
+    state = torch.full((3, 64), 2.0, device="cuda")
+    step = lambda s: _cv().gated_linear_recurrence_update(s, x, f, None, lower)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(state.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(256):
+            step(state)
+    for _ in range(length // 256):
+        graph.replay()
+    want = 0.5 + 1.5 * decay[-1]
+    assert bool(((state.double().cpu() - want).abs() <= 1e-4 * 2).all()), float((state.double().cpu() - want).abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 33])
+def test_forgotten_states_keep_their_digits(dim, dtype):
+    """x = 0: the state is the product of the gates, down to 1e-30 of where it began; each of a product's
+    n factors errs by 2 eta g / a and a rounding, 2e-6 n at gates of 0.95 and below."""
+    length = 1200
+    f = torch.full((1, length, dim), 3.0, dtype=dtype)
+    x = torch.zeros_like(f)
+    init = torch.linspace(0.5, 2, dim)[None]
+    y, final = _cv().gated_linear_recurrence(x.cuda(), f.cuda(), initial_state=init.cuda())
+    want = init.double() * torch.sigmoid(torch.tensor(3.0, dtype=torch.float64)) ** length
+    assert float(want.min()) < 1e-25 and bool(((final.double().cpu() - want).abs() <= 2e-6 * length * want).all())
+    cv, state = _cv(), init.cuda()
+    for _ in range(length):
+        cv.gated_linear_recurrence_update(state, x[:, 0].cuda(), f[:, 0].cuda())
+    assert bool(((state.double().cpu() - want).abs() <= 2e-6 * length * want).all())
+
+
+@pytest.mark.gpu
+def test_states_that_are_infinite_stay_so():
+    """An infinite input or state: a h + g x stays infinite with every open gate, and a reset clears it."""
+    cv = _cv()
+    for batch, length, dim in ((1, 900, 64), (40, 900, 1024)):
+        x = torch.zeros(batch, length, dim, device="cuda")
+        x[:, 3, 0], x[:, 700, 1] = float("inf"), -float("inf")
+        f = torch.full_like(x, 9.0)
+        init = torch.zeros(batch, dim, device="cuda")
+        init[:, 2] = float("inf")
+        y, final = cv.gated_linear_recurrence(x, f, initial_state=init)
+        assert bool((y[:, 3:, 0] == float("inf")).all()) and bool((y[:, 700:, 1] == -float("inf")).all())
+        assert bool((y[:, :, 2] == float("inf")).all()) and bool((y[:, :, 3:] == 0).all())
+        reset = torch.zeros(batch, length, dtype=torch.bool, device="cuda")
+        reset[:, 800] = True
+        y, final = cv.gated_linear_recurrence(x, f, initial_state=init, reset=reset)
+        assert bool((y[:, 800:] == 0).all()) and bool((final == 0).all()) and bool((y[:, 799, :3].isinf()).all())
+    state = torch.tensor([[float("inf"), -float("inf"), 1e10, 3.0]], device="cuda")
+    x = torch.ones_like(state)
+    cv.gated_linear_recurrence_update(state, x, torch.tensor([[2.0, 20.0, -80.0, float("inf")]], device="cuda"))
+    assert state.tolist() == [[float("inf"), -float("inf"), 1.0, 3.0]]
+
+
+@pytest.mark.gpu
+def test_lower_bounds_outside_their_range_follow_the_formula():
+    """A bound that training has pushed slightly past 0 or 1: the factor 1 - g may be negative or above one."""
+    t = _make(2, 300, 64, F32, False, True, True, False, spread=30.0)
+    t["lower"] = torch.linspace(-0.05, 1.0005, 64)
+    y, final = _cv().gated_linear_recurrence(*(t[k].cuda() if k in t else None for k in ("x", "forget", "z", "lower", "init")))
+    want, last = lm.gated_recurrence_ref(*(t[k].double() if k in t else None for k in ("x", "forget", "z", "lower", "init")))
+    m = float(max(t["x"].abs().max(), t["init"].abs().max(), want.abs().max()))
+    assert float((y.double().cpu() - want).abs().max()) <= C * m
+    assert float((final.double().cpu() - last).abs().max()) <= C * m
