@@ -32,8 +32,8 @@
 // ring of shared-memory stages filled ahead: by TMA, by 4-byte asynchronous copies
 // where rows do not start on 16-byte boundaries; odd widths of 16-bit data are
 // read directly.
-// A composition whose A is exactly 0 (a reset) takes H alone: a state that is not
-// finite does not pass a reset.
+// A composition whose A is exactly 0 (a reset) takes H alone: neither a state that is not
+// finite nor a NaN gate passes a reset, forward or backward.
 // The forward saves the state that enters each chunk, in fp32, for the backward,
 // which recomputes the chunk's states from it.
 #include <cooperative_groups.h>
@@ -308,9 +308,17 @@ __device__ __forceinline__ void again(float2 (&v)[N]) {
 }
 
 template <typename F> struct Map { F A, H; };
+// Factors joined: with resets, 0 whatever the other factor is (a gate may be NaN).
+template <bool RESET>
+__device__ __forceinline__ float joined(float A, float B) { return RESET && (A == 0.0f || B == 0.0f) ? 0.0f : A * B; }
+template <bool RESET>
+__device__ __forceinline__ float2 joined(float2 A, float2 B) {
+    if constexpr (!RESET) return mul2(A, B);
+    return make_float2(joined<true>(A.x, B.x), joined<true>(A.y, B.y));
+}
 template <bool RESET, typename F>
 __device__ __forceinline__ Map<F> then(const Map<F>& first, const Map<F>& next) {
-    return {mu(first.A, next.A), through<RESET>(next.A, next.H, first.H)};
+    return {joined<RESET>(first.A, next.A), through<RESET>(next.A, next.H, first.H)};
 }
 
 // A product A of factors near one is known to 2^-24 of itself a factor, and with steady gates the
@@ -478,6 +486,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
                 m.A = mu(m.A, av[i]);
             }
         }
+        if (RESET && rs) m.A = same<F>(0.0f);             // also where a later gate is NaN
         settle(m.A, lacking(m.A, B), left);
         Map<F>(*mw)[32] = maps[n & 1];
         mw[warp][lane] = m;
@@ -632,6 +641,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
             m.H = fm(av, m.H, mu(g, unpack<T>(xw[i])));
             m.A = mu(m.A, av);
         }
+        if (RESET && rs) m.A = same<F>(0.0f);             // also where a later gate is NaN
         settle(m.A, lacking(m.A, B), left);
         F d = zero;
 #pragma unroll

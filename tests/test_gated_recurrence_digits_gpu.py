@@ -310,3 +310,36 @@ def test_lower_bounds_outside_their_range_follow_the_formula():
     m = float(max(t["x"].abs().max(), t["init"].abs().max(), want.abs().max()))
     assert float((y.double().cpu() - want).abs().max()) <= C * m
     assert float((final.double().cpu() - last).abs().max()) <= C * m
+
+
+# ------------------------------------------------------- gates that are not numbers --
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("batch,dim", [(1, 64), (1, 33), (40, 1024)])
+@pytest.mark.parametrize("at", [3, 130, 255, 256, 260, 399])
+def test_nan_gates_do_not_cross_a_reset(batch, dim, dtype, at):
+    """Packed sequences [0, 256), [256, 400), [400, 700): a NaN gate in one (or NaN gradients) leaves the outputs
+    of those after it and the gradients of those before it as they are without it, bit for bit."""
+    length, cuts = 700, [0, 256, 400]
+    g = torch.Generator().manual_seed(at)
+    x, f, z = (torch.randn(batch, length, dim, generator=g).to(dtype).cuda() for _ in range(3))
+    reset = torch.zeros(batch, length, dtype=torch.bool)
+    reset[:, cuts] = True
+    reset = reset.cuda()
+    dy, df = torch.randn(batch, length, dim, generator=g).to(dtype).cuda(), torch.randn(batch, dim, generator=g).cuda()
+    bad = f.clone()
+    bad[:, at, 3] = float("nan")
+    runs = []
+    for gates in (f, bad):
+        leaves = [t.clone().requires_grad_(True) for t in (x, gates, z)]
+        y, final = _cv().gated_linear_recurrence(*leaves, reset=reset)
+        runs.append([y.detach(), final.detach(), *torch.autograd.grad((y, final), leaves, (dy, df))])
+    begin, end = (0, 256) if at < 256 else (256, 400)
+    for a, b in zip(*runs):
+        if a.dim() == 2:
+            assert torch.equal(a, b)
+            continue
+        assert torch.equal(a[:, :begin], b[:, :begin]) and torch.equal(a[:, end:], b[:, end:])
+        other = torch.arange(dim, device="cuda") != 3
+        assert torch.equal(a[..., other], b[..., other])
+    assert bool(runs[1][0][:, at, 3].isnan().all())
