@@ -354,13 +354,28 @@ def direct(*tensors) -> bool:
     """Whether a call may go to the library itself (with a gradient: through a
     ``torch.autograd.Function``) instead of the custom op of torch's dispatcher:
     the tensors are plain ones (no fake or other subclass) on the current
-    device, and nothing is being traced.  The
+    device, and nothing watches the dispatcher (:func:`watched`).  The
     dispatcher's Python path costs about 15 us a call, more than the kernels
     of a decode step run for."""
     for t in tensors:
         if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
             return False
-    return not torch.compiler.is_compiling() and tensors[0].get_device() == torch._C._cuda_getDevice()
+    return not watched() and tensors[0].get_device() == torch._C._cuda_getDevice()
+
+
+def watched() -> bool:
+    """Whether something has to see the call as an operator of torch's dispatcher:
+    ``torch.compile``, ``torch.jit.trace``, a dispatch mode (``make_fx``, fake tensors,
+    logging and counting modes) or a functorch transform (``vmap``).  Their tensors may
+    look plain, and a launch beside the dispatcher would leave them with memory that the
+    recorded program never writes.  0.3 us."""
+    return (torch.compiler.is_compiling() or _is_tracing() or _dispatch_modes() > 0
+            or _functorch_level() is not None)
+
+
+_is_tracing = torch._C._is_tracing
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_functorch_level = torch._C._functorch.maybe_current_level
 
 
 def wants_grad(*tensors) -> bool:
