@@ -297,5 +297,8 @@ def gated_linear_recurrence_update(state, x, forget, z=None, lower_bound=None):
 
     x, forget, z, lower = _rows(x), _rows(forget), _rows(z), _f32(lower_bound)
     if nat.direct(x, state, forget, z, lower):
-        return _update(state, x, forget, z, lower)
+        y = _update(state, x, forget, z, lower)
+        if not state.is_inference():                # autograd sees the change, as the registered op shows it
+            torch.autograd.graph.increment_version(state)
+        return y
     return torch.ops.b200ssm.gated_recurrence_update(state, x, forget, z, lower)
