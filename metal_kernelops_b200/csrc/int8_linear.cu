@@ -24,6 +24,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <mutex>
@@ -133,6 +134,9 @@ struct Skinny {
     static size_t smem(int stages) { return (size_t)stages * kStage + 1024; }
     // the sums pass through the stages' memory
     static int min_stages() { return (NT * kFeatures * 4 + kStage - 1) / kStage; }
+    // where the choice of stages begins (about 72 KB) and ends
+    static int first_stages() { return std::max({min_stages(), 2, (72 << 10) / kStage}); }
+    static int last_stages() { return std::max(first_stages(), std::min(kMaxStages, (200 << 10) / kStage)); }
 };
 
 // Grid: (feature tiles * C, token tiles); a cluster's C CTAs share a tile, each with
@@ -570,13 +574,15 @@ static int launch_skinny(TmaArgs& ta, cudaStream_t st) {
     // clusters has to wait; 11.5 us uncut.
     const int64_t tiles = ftiles * mtiles;
     auto fits = [&](int s, int c) { return tiles <= clusters_at_once<O, NT>(s, c); };
-    const int least = (int)max64(L::min_stages(), 2);
-    int S = (int)max64(least, (72 << 10) / L::kStage), C = 1;
+    int S = L::first_stages(), C = 1;
     while (C < 8 && blocks >= 2 * (C + 1) && fits(S, C + 1)) ++C;
-    while (S < kMaxStages && (int64_t)S * C < blocks && (size_t)(S + 1) * L::kStage <= (200 << 10) && fits(S + 1, C)) ++S;
+    while (S < L::last_stages() && (int64_t)S * C < blocks && fits(S + 1, C)) ++S;
     ta.stages = S;
     const size_t smem = L::smem(ta.stages);
-    if (cudaFuncSetAttribute(skinny_kernel<O, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    // the limit belongs to the kernel, not to this call: one value for every call, so that
+    // another thread's cannot lower it before this launch
+    if (cudaFuncSetAttribute(skinny_kernel<O, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)L::smem(L::last_stages())) != cudaSuccess)
         return check_launch("int8_linear");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(ftiles * C), (unsigned)mtiles);
