@@ -180,19 +180,23 @@ skinny_kernel(const __grid_constant__ TmaArgs ta) {
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_at;
+    int loads = nk < stages ? nk : stages;              // thread 0's, so far
+    bool ok = true;
     if (warp == 0 && lane == 0) {
-        for (int i = stages; i < nk; ++i) {
-            if (!tc::mbar_wait(tc::smem_u32(&empty[i % stages]), (uint32_t)(i / stages - 1) & 1u)) {
+        for (; loads < nk; ++loads) {
+            if (!tc::mbar_wait(tc::smem_u32(&empty[loads % stages]), (uint32_t)(loads / stages - 1) & 1u)) {
                 report(a, 121);
+                ok = false;
                 break;
             }
-            load(i);
+            load(loads);
         }
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < nk; ++i) {
             const int s = i % stages;
             if (!tc::mbar_wait(tc::smem_u32(&full[s]), (uint32_t)(i / stages) & 1u)) {
                 report(a, 122);
+                ok = false;
                 break;
             }
             tc::fence_after();
@@ -206,11 +210,18 @@ skinny_kernel(const __grid_constant__ TmaArgs ta) {
         tc::commit(tc::smem_u32(&done));
     }
     __syncwarp();
-    const bool ok = tc::mbar_wait(tc::smem_u32(&done), 0);
-    if (!ok && lane == 0) report(a, 123);
+    if (!tc::mbar_wait(tc::smem_u32(&done), 0)) {
+        if (lane == 0) report(a, 123);
+        ok = false;
+    }
+    // a wait has given up: no copy may land in a CTA that has ended, and nothing is written
+    ok = __syncthreads_and(ok);
+    if (!ok && threadIdx.x == 0)
+        for (int i = loads > stages ? loads - stages : 0; i < loads; ++i)
+            tc::mbar_wait(tc::smem_u32(&full[i % stages]), (uint32_t)(i / stages) & 1u);
     tc::fence_after();
     // tensor memory (lane: feature, column: token) to shared memory (token, feature)
-    const int live = (int)min64(NT, a.tokens - m0);
+    const int live = ok ? (int)min64(NT, a.tokens - m0) : 0;
     int* part = reinterpret_cast<int*>(smem);
     for (int c0 = 0; c0 < live; c0 += 16) {
         int acc[16];
@@ -382,8 +393,12 @@ wide_kernel(const __grid_constant__ TmaArgs ta) {
         for (int64_t i = max64(0, it - kWideStages); ok && i < it; ++i)
             if (!tc::mbar_wait(tc::smem_u32(&empty[i % kWideStages]), (uint32_t)(i / kWideStages) & 1u)) {
                 report(a, 132);
-                break;
+                ok = false;
             }
+        // a wait has given up: the pair's copies, which count on the first CTA's barriers, land before either ends
+        if (!ok && rank == 0)
+            for (int64_t i = max64(0, it - kWideStages); i < it; ++i)
+                tc::mbar_wait(tc::smem_u32(&full[i % kWideStages]), (uint32_t)(i / kWideStages) & 1u);
     } else if (warp == 1 && lane == 0 && rank == 0) {
         int64_t it = 0;
         int64_t n = 0;
