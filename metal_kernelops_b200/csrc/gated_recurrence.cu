@@ -89,6 +89,20 @@ __device__ __forceinline__ void report(const Args& a, int code) {
     if (a.status) atomicCAS(a.status, 0, code);
 }
 
+// A bounded wait of a CTA, for at most `polls` tries.  One that gives up leaves the others a single
+// try: from then on no more copies are asked for and no more maps sent, so that the CTA gets to its
+// end, where what is on its way still has the time of a whole wait to land.
+constexpr uint32_t kPolls = 1u << 22;
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile uint32_t* polls) {
+    const bool ok = tc::mbar_wait(bar, parity, *polls);
+    if (!ok) *polls = 1;
+    return ok;
+}
+__device__ __forceinline__ void let_land(uint32_t bar) {
+    if (threadIdx.x == 0)
+        for (uint32_t parity = 0; parity < 2; ++parity) tc::mbar_wait(bar, parity);
+}
+
 // ------------------------------------------------- one or two channels a lane --
 template <typename T> struct Lane { using F = float2; static constexpr int E = 2; };
 template <> struct Lane<float> { using F = float; static constexpr int E = 1; };
@@ -223,13 +237,15 @@ __device__ __forceinline__ void st_chan(float* p, int64_t c, int64_t dim, float2
     if (c + 1 < dim) p[c + 1] = v.y;
 }
 
-// Bit i: the i-th of the warp's N steps (from t) is a reset.
+// Whether the lane's one of the warp's N steps (from t) is a reset.  The warp votes on it where the mask is
+// used, so that the load's time passes beside the gates'.
 template <int N>
-__device__ __forceinline__ uint32_t reset_mask(const uint8_t* reset, int64_t row, int64_t t, int64_t length) {
+__device__ __forceinline__ uint8_t reset_at(const uint8_t* reset, int64_t row, int64_t t, int64_t length) {
     const int lane = threadIdx.x & 31;
-    const bool r = lane < N && t + lane < length && reset[row + t + lane] != 0;
-    return __ballot_sync(0xffffffffu, r);
+    return lane < N && t + lane < length ? reset[row + t + lane] : (uint8_t)0;
 }
+// Bit i: step i is a reset.
+__device__ __forceinline__ uint32_t reset_mask(uint8_t at) { return __ballot_sync(0xffffffffu, at != 0); }
 
 template <typename T, int N>
 __device__ __forceinline__ void ld_steps(const void* base, int64_t row, int64_t stride, int64_t t, int live, int64_t c,
@@ -263,6 +279,9 @@ struct Ring {
         tc::mbar_expect_tx(bar(s), NT * kTile);
         for (int i = 0; i < NT; ++i)
             tc::tma_load3(tc::smem_u32(base + (s * NT + i) * kTile), &ta.m[which[i]], c0, (int)t, b, bar(s));
+    }
+    __device__ __forceinline__ void drain() const {
+        for (int s = 0; s < ST; ++s) let_land(bar(s));
     }
     // The lane's words of tensor i: N steps from p, `live` of them inside the sequence.
     template <typename T>
@@ -386,17 +405,20 @@ struct alignas(128) Exchange {        // whole 128-byte lines: the ring behind i
         }
     }
     // One warp: its lanes' maps of the whole chunk to every CTA.
-    __device__ __forceinline__ void put(int64_t round, int rank, int C, const Map<F>& all) {
-        const int s = (int)(round & 1);
+    __device__ __forceinline__ void put(int round, int rank, int C, const Map<F>& all) {
+        const int s = round & 1;
         const uint32_t at = tc::smem_u32(&far[s][rank][threadIdx.x & 31]), bar = tc::smem_u32(&bars[s]);
         for (int r = 0; r < C; ++r) send(remote(at, r), remote(bar, r), all.A, all.H);
     }
     // Every thread: the round's maps are here.
-    __device__ __forceinline__ bool wait(int64_t round, int C) {
-        const int s = (int)(round & 1);
-        const bool ok = tc::mbar_wait(tc::smem_u32(&bars[s]), (uint32_t)(round >> 1) & 1u);
+    __device__ __forceinline__ bool wait(int round, int C, volatile uint32_t* polls) {
+        const int s = round & 1;
+        if (!wait_for(tc::smem_u32(&bars[s]), (uint32_t)(round >> 1) & 1u, polls)) return false;
         if (threadIdx.x == 0) arm(s, C);
-        return ok;
+        return true;
+    }
+    __device__ __forceinline__ void drain() {
+        for (int s = 0; s < 2; ++s) let_land(tc::smem_u32(&bars[s]));
     }
 };
 __device__ __forceinline__ int cluster_size() { return (int)cooperative_groups::this_cluster().num_blocks(); }
@@ -409,6 +431,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     const Args& a = ta.a;
     __shared__ Map<F> maps[2][kWarps][32];
     __shared__ Exchange<F> ex;
+    __shared__ volatile uint32_t polls;
     extern __shared__ __align__(128) uint8_t smem[];
     const Ring<NT, ST, N> ring{smem};
     const int which[3] = {0, 1, 2};
@@ -416,20 +439,23 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     const int C = cluster_size(), rank = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.y, tile = blockIdx.x / C, c = (tile * 32 + lane) * E;
-    const int64_t rounds = (a.chunks + C - 1) / C;
+    // tokens, chunks and rounds fit 31 bits, a last chunk's overhang included
+    const int rounds = (int)((a.chunks + C - 1) / C);
+    if (threadIdx.x == 0) polls = kPolls;
+    __syncthreads();
     if (C > 1) {
         ex.init(C);
         cluster.sync();                                 // every CTA's barriers are there to write to
     }
     // the chunk of round n into its stage
-    auto fill = [&](int64_t n) {
-        const int s = (int)(n % ST);
-        const int64_t t0 = (n * C + rank) * kChunk;
+    auto fill = [&](int n) {
+        const int s = n % ST;
+        const int t0 = (n * C + rank) * kChunk;
         if constexpr (LOADS == kTma) {
-            if (threadIdx.x == 0) ring.load(ta, s, (int)(tile * 32 * E), t0, (int)b, which);
+            if (threadIdx.x == 0 && polls == kPolls) ring.load(ta, s, (int)(tile * 32 * E), t0, (int)b, which);
         } else if constexpr (LOADS == kWords) {
-            const int64_t t = t0 + warp * N;
-            const int live = (int)max64(0, min64(N, a.length - t));
+            const int t = t0 + warp * N;
+            const int live = max(0, min(N, (int)a.length - t));
             ring.template copy<T>(s, 0, a.x, b * a.xb, a.xt, t, live, c, a.dim);
             ring.template copy<T>(s, 1, a.forget, b * a.fb, a.ft, t, live, c, a.dim);
             if (GATE) ring.template copy<T>(s, 2, a.z, b * a.zb, a.zt, t, live, c, a.dim);
@@ -446,20 +472,21 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
     span = sub(same<F>(1.0f), span);
     ld_chan(a.init ? a.init + b * a.dim : nullptr, c, a.dim, 0.0f, S);
     F left = same<F>(0.0f), left_all = same<F>(0.0f);
-    for (int64_t n = 0; n < rounds; ++n) {
-        const int64_t chunk = n * C + rank, t = chunk * kChunk + warp * N;
-        const int live = (int)max64(0, min64(N, a.length - t));
+    for (int n = 0; n < rounds; ++n) {
+        const int chunk = n * C + rank, t = chunk * kChunk + warp * N;
+        const int live = max(0, min(N, (int)a.length - t));
         uint32_t zw[N];
         F av[N], bv[N];                   // h -> av h + bv
         Map<F> m{same<F>(1.0f), same<F>(0.0f)};
         F B = same<F>(0.0f);              // 1 - m.A, added up
-        const uint32_t rs = RESET ? reset_mask<N>(a.reset, b * a.length, t, a.length) : 0u;
+        uint32_t rs = 0;                  // the resets among the steps
+        const uint8_t reset = RESET ? reset_at<N>(a.reset, b * a.length, t, a.length) : (uint8_t)0;
         {
             uint32_t xw[N], fw[N];
             if constexpr (LOADS != kDirect) {
-                const int s = (int)(n % ST);
+                const int s = n % ST;
                 if constexpr (LOADS == kTma) {
-                    if (!tc::mbar_wait(ring.bar(s), (uint32_t)(n / ST) & 1u) && lane == 0) report(a, 111);
+                    if (!wait_for(ring.bar(s), (uint32_t)(n / ST) & 1u, &polls)) report(a, 111);
                 } else {
                     tc::cp_async_wait<ST - 1>();
                 }
@@ -471,6 +498,7 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
                 ld_steps<T, N>(a.forget, b * a.fb, a.ft, t, live, c, a, fw);
                 if (GATE) ld_steps<T, N>(a.z, b * a.zb, a.zt, t, live, c, a, zw);
             }
+            if (RESET) rs = reset_mask(reset);
             if (live < N) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) fw[i] = i < live ? fw[i] : kKeep<T>;
@@ -515,9 +543,9 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
                 for (int w = 0; w < kWarps - 1; ++w) before = then<RESET>(before, mw[w][lane], lacks);
                 Map<F> all = then<RESET>(before, m, lacks);
                 settle(all.A, lacks, left_all);
-                ex.put(n, rank, C, all);
+                if (polls == kPolls) ex.put(n, rank, C, all);
             }
-            if (!ex.wait(n, C) && lane == 0) report(a, 113);
+            if (!ex.wait(n, C, &polls)) report(a, 113);
             h = S;
 #pragma unroll
             for (int r = 0; r < kMaxCluster; ++r) {
@@ -546,7 +574,11 @@ fwd_kernel(const __grid_constant__ TmaArgs ta) {
             y.move(a.dim);
         }
     }
-    if (C > 1) cluster.sync();                          // nothing is on its way to a CTA that ends
+    if (LOADS == kTma && polls != kPolls) ring.drain();
+    if (C > 1) {
+        cluster.sync();                                 // nothing is on its way to a CTA that ends
+        if (polls != kPolls) ex.drain();
+    }
     if (warp == 0 && rank == 0) st_chan(a.final_state + b * a.dim, c, a.dim, S);
 }
 
@@ -558,6 +590,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
     const Args& a = ta.a;
     __shared__ struct { Map<F> m[32]; F R[32]; } maps[2][kWarps];
     __shared__ Exchange<F> ex;            // of (A, R)
+    __shared__ volatile uint32_t polls;
     __shared__ F sums[kWarps][32];
     extern __shared__ __align__(128) uint8_t smem[];
     const Ring<NT, ST, N> ring{smem};
@@ -566,20 +599,23 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
     const int C = cluster_size(), rank = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.y, tile = blockIdx.x / C, c = (tile * 32 + lane) * E;
-    const int64_t rounds = (a.chunks + C - 1) / C;
+    // tokens, chunks and rounds fit 31 bits, a last chunk's overhang included
+    const int rounds = (int)((a.chunks + C - 1) / C);
+    if (threadIdx.x == 0) polls = kPolls;
+    __syncthreads();
     if (C > 1) {
         ex.init(C);
         cluster.sync();                                 // every CTA's barriers are there to write to
     }
     // the chunk of a turn into its stage
-    auto fill = [&](int64_t turn) {
-        const int s = (int)(turn % ST);
-        const int64_t t0 = ((rounds - 1 - turn) * C + rank) * kChunk;
+    auto fill = [&](int turn) {
+        const int s = turn % ST;
+        const int t0 = ((rounds - 1 - turn) * C + rank) * kChunk;
         if constexpr (LOADS == kTma) {
-            if (threadIdx.x == 0) ring.load(ta, s, (int)(tile * 32 * E), t0, (int)b, which);
+            if (threadIdx.x == 0 && polls == kPolls) ring.load(ta, s, (int)(tile * 32 * E), t0, (int)b, which);
         } else if constexpr (LOADS == kWords) {
-            const int64_t t = t0 + warp * N;
-            const int live = (int)max64(0, min64(N, a.length - t));
+            const int t = t0 + warp * N;
+            const int live = max(0, min(N, (int)a.length - t));
             ring.template copy<T>(s, 0, a.x, b * a.xb, a.xt, t, live, c, a.dim);
             ring.template copy<T>(s, 1, a.forget, b * a.fb, a.ft, t, live, c, a.dim);
             ring.template copy<T>(s, 2, a.dy, b * a.dyb, a.dyt, t, live, c, a.dim);
@@ -598,19 +634,19 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
     span = sub(one, span);
     ld_chan(a.dfinal ? a.dfinal + b * a.dim : nullptr, c, a.dim, 0.0f, D);
     F dlower = zero, left = zero, left_all = zero;
-    for (int64_t turn = 0; turn < rounds; ++turn) {
-        const int64_t chunk = (rounds - 1 - turn) * C + rank, t = chunk * kChunk + warp * N;
-        const int live = (int)max64(0, min64(N, a.length - t));
+    for (int turn = 0; turn < rounds; ++turn) {
+        const int chunk = (rounds - 1 - turn) * C + rank, t = chunk * kChunk + warp * N;
+        const int live = max(0, min(N, (int)a.length - t));
         uint32_t xw[N], zw[N], dw[N];
         F ev[N], h;                       // e^forget
-        const uint32_t rs = RESET ? reset_mask<N>(a.reset, b * a.length, t, a.length) : 0u;
+        const uint8_t reset = RESET ? reset_at<N>(a.reset, b * a.length, t, a.length) : (uint8_t)0;
         ld_chan(chunk < a.chunks ? a.states + (b * a.saved + chunk) * a.dim : nullptr, c, a.dim, 0.0f, h);
         {
             uint32_t fw[N];
             if constexpr (LOADS != kDirect) {
-                const int s = (int)(turn % ST);
+                const int s = turn % ST;
                 if constexpr (LOADS == kTma) {
-                    if (!tc::mbar_wait(ring.bar(s), (uint32_t)(turn / ST) & 1u) && lane == 0) report(a, 112);
+                    if (!wait_for(ring.bar(s), (uint32_t)(turn / ST) & 1u, &polls)) report(a, 112);
                 } else {
                     tc::cp_async_wait<ST - 1>();
                 }
@@ -631,6 +667,7 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
 #pragma unroll
             for (int i = 0; i < N; ++i) ev[i] = exp_of(unpack<T>(fw[i]));
         }
+        const uint32_t rs = RESET ? reset_mask(reset) : 0u;
         Map<F> m{one, zero};
         F B = zero;                                     // 1 - m.A, added up
 #pragma unroll
@@ -680,9 +717,9 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
                     after = then<RESET>(after, Map<F>{mw[w].m[lane].A, mw[w].R[lane]}, lacks);
                 Map<F> all = then<RESET>(after, Map<F>{m.A, d}, lacks);
                 settle(all.A, lacks, left_all);
-                ex.put(turn, rank, C, all);
+                if (polls == kPolls) ex.put(turn, rank, C, all);
             }
-            if (!ex.wait(turn, C) && lane == 0) report(a, 114);
+            if (!ex.wait(turn, C, &polls)) report(a, 114);
             d = D;
 #pragma unroll
             for (int r = kMaxCluster - 1; r >= 0; --r) {
@@ -742,7 +779,11 @@ bwd_kernel(const __grid_constant__ TmaArgs ta) {
         }
         dlower = ad(dlower, dl);
     }
-    if (C > 1) cluster.sync();                          // nothing is on its way to a CTA that ends
+    if (LOADS == kTma && polls != kPolls) ring.drain();
+    if (C > 1) {
+        cluster.sync();                                 // nothing is on its way to a CTA that ends
+        if (polls != kPolls) ex.drain();
+    }
     if (warp == 0 && rank == 0 && a.dinit != nullptr) st_chan(a.dinit + b * a.dim, c, a.dim, D);
     if (a.part != nullptr) {
         sums[warp][lane] = dlower;
