@@ -193,7 +193,7 @@ def _backward(ctx, dy, dstream, drstd):
     dstream = _rows(dstream, stream.shape[1]) if ctx.residual and dstream is not None else None
     dy = torch.zeros(stream.shape, dtype=ctx.xdtype, device=stream.device) if dy is None else _rows(dy, stream.shape[1])
     dx, dres, dw = _bwd(dy, dstream, stream, weight, rstd, ctx.eps)
-    dres = None if not ctx.residual else dres if dres.numel() or not dx.numel() else dx
+    dres = None if not ctx.residual else dx if stream.dtype == dx.dtype else dres
     return dx, dw.to(weight.dtype), dres, None, None
 
 
@@ -260,10 +260,10 @@ def add_rmsnorm(x, weight, residual=None, eps=1e-5):
         without a residual).
     """
     _check("add_rmsnorm", x, weight, residual)
-    if x.numel() == 0:
-        return x.new_empty(x.shape), x if residual is None else x + residual
-    w = weight if weight.is_contiguous() else weight.contiguous()
     grad = nat.wants_grad(x, weight, residual)
+    if x.numel() == 0 and not grad:
+        return x.new_empty(x.shape), x if residual is None else x.new_empty(x.shape, dtype=residual.dtype)
+    w = weight if weight.is_contiguous() else weight.contiguous()
     if nat.direct(x, w, residual):
         if grad:
             out = _AddRmsNorm.apply(x, w, residual, float(eps))
@@ -285,7 +285,7 @@ def add_rmsnorm_int8(x, weight, residual=None, eps=1e-5):
         raise ValueError("add_rmsnorm_int8 has no gradient: call it under torch.no_grad(), or use add_rmsnorm")
     if x.numel() == 0:
         return (x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32),
-                x if residual is None else x + residual)
+                x if residual is None else x.new_empty(x.shape, dtype=residual.dtype))
     w = weight if weight.is_contiguous() else weight.contiguous()
     if nat.direct(x, w, residual):
         q, scale, stream = _forward_int8(_features(x), w, None if residual is None else _features(residual),
