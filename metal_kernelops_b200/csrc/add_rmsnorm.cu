@@ -359,7 +359,7 @@ bwd_kernel(const Args a) {
                 const int64_t e = ((int64_t)k * tx + threadIdx.x) * V;
                 if (e < F) {
                     sr[k].ld(s + row * a.xs + e);
-                    if (dy) dyr[k].ld(dy + row * a.dys + e);
+                    dyr[k].ld(dy + row * a.dys + e);
                     if (ds) dsr[k].ld(ds + row * a.dss + e);
                 }
             }

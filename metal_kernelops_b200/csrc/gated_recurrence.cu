@@ -11,9 +11,9 @@
 // k_t is 1 / (1 + e^forget): the complement of the gate is computed as such, so that g of
 // gates near one (long memory) keeps its digits.  e^forget is two to a rounded product, so g and
 // k err by up to (1.25 |forget| + 10) 2^-24 of themselves.  a = 1 - g is rounded to
-// 2^-25; what the products of a row lack by that is carried along (settle()), which costs an
-// addition a step: 16 x 4096 x 5120 bf16 with gate 423 us as before, the backward 898 -> 915; 1 x 4096 x 5120
-// 44 -> 45 and 87 -> 92.  Without it a steady forget of 8 over 65536 steps ended 1e-3 off.
+// 2^-25; what the products of a row lack by that is carried along (settle()), which costs a
+// fused addition a step (2 % of the backward).  Without it a steady forget of 8 with a lower
+// bound of 0.9 ended 1e-3 off after 65536 steps, with it 5e-6.
 // Backward, with dh_t the gradient of h_t and a_t taken as 0 at a reset:
 //     dh_t = dy_t silu(z_t) + a_{t+1} dh_{t+1}   (+ dfinal at the last step)
 //     dx = g dh,  dg = dh (x - h'),  dforget = -dg g (1 - k),  dlower = -sum dg k,  1 - k = k e^forget
@@ -53,9 +53,9 @@ namespace glr {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 // A warp's steps of a chunk.  The forward holds 16 (its two factors a step and z fill
-// the 128 registers of two CTAs per SM): 1 x 4096 x 2560 bf16 with gate takes 31 us, 37
-// with 8 and three CTAs per SM, whose exchange comes twice as often.  The backward
-// holds more for a step, so 8.
+// the 128 registers of two CTAs per SM): 2 x 16384 x 5120 bf16 with gate takes 271 us, 313
+// with 8 and three CTAs per SM, whose exchange comes twice as often; 16 x 4096 x 5120 416
+// and 431.  The backward holds more for a step, so 8.
 constexpr int kFwdSteps = 16, kBwdSteps = 8;
 constexpr int kMaxCluster = 8;
 constexpr int kRow = 128;                           // bytes of a step of one tensor
@@ -938,9 +938,9 @@ static bool tma_ok(const Args& a, int dtype, bool bwd) {
 // tiles run in as many waves as the GPU's room for such clusters needs; a round of a
 // cluster costs 12 % and 6 % more per CTA than a lone CTA's (the exchange, and the
 // spread of its CTAs).  The C with the least product is taken.  Measured, forward, bf16
-// with gate, room for 296 CTAs: 1 x 4096 x 5120 (80 tiles) 59 us with C = 1, 45 with 3,
-// 51 with 4; 2 x 16384 x 5120 (160 tiles) 365 us with 1, 309 with 2, 264 with 4, 299
-// with 8; 16 x 4096 x 5120 (1280 tiles) 411 us with 1, 451 with 2.
+// with gate, room for 296 CTAs: 1 x 4096 x 5120 (80 tiles) 57 us with C = 1, 43 with 3,
+// 50 with 4; 2 x 16384 x 5120 (160 tiles) 356 us with 1, 328 with 2, 271 with 4, 301
+// with 8; 16 x 4096 x 5120 (1280 tiles) 416 us with 1, 470 with 2.
 template <auto kernel>
 static int cluster_of(int64_t tiles, int64_t chunks, size_t smem) {
     static std::atomic<int> room[kMaxCluster + 1]; // clusters that fit at once, by size; 0: not asked yet

@@ -645,8 +645,10 @@ static int launch_wide(TmaArgs& ta, cudaStream_t st) {
     return check_launch("int8_linear");
 }
 
-// From this many tokens on the wide kernel runs: at 256 x 2560 -> 12368 the skinny one
-// takes 20.7 us and the wide one 21.5, at 400 28.0 and 21.6.
+// From this many tokens on the wide kernel runs: with 2560 -> 12368, whose tiles fill the
+// GPU, the skinny one takes 19.4 us at 256 tokens, 22.8 at 257 and 26.4 at 400, the wide one 18.2 at 257 and 19.9 at
+// 400.  Narrow layers, whose tiles do not, would do better with the skinny one for longer: 300 x 5120
+// -> 2560 14.5 us (wide 17.9), 512 tokens 16.8 (18.2), 1024 tokens 24.0 (18.3); 300 x 8192 -> 256 10.8 (24.9).
 constexpr int64_t kWideTokens = 257;
 
 }  // namespace i8
