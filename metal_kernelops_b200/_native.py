@@ -354,25 +354,20 @@ def direct(*tensors) -> bool:
     """Whether a call may go to the library itself (with a gradient: through a
     ``torch.autograd.Function``) instead of the custom op of torch's dispatcher:
     the tensors are plain ones (no fake or other subclass) on the current
-    device, and nothing watches the dispatcher (:func:`watched`).  The
-    dispatcher's Python path costs about 15 us a call, more than the kernels
-    of a decode step run for."""
+    device, and nothing has to see the call as an operator: ``torch.compile``,
+    ``torch.jit.trace``, a dispatch mode (``make_fx``, fake tensors, logging and
+    counting modes) or a functorch transform (``vmap``).  Their tensors may look plain,
+    and a launch beside the dispatcher would leave them with memory that the
+    recorded program never writes.  The dispatcher's Python path costs about 15 us
+    a call, more than the kernels of a decode step run for."""
     for t in tensors:
         if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
             return False
-    return not watched() and tensors[0].get_device() == torch._C._cuda_getDevice()
+    return not (_is_compiling() or _is_tracing() or _dispatch_modes() or _functorch_level() is not None) \
+        and tensors[0].get_device() == torch._C._cuda_getDevice()
 
 
-def watched() -> bool:
-    """Whether something has to see the call as an operator of torch's dispatcher:
-    ``torch.compile``, ``torch.jit.trace``, a dispatch mode (``make_fx``, fake tensors,
-    logging and counting modes) or a functorch transform (``vmap``).  Their tensors may
-    look plain, and a launch beside the dispatcher would leave them with memory that the
-    recorded program never writes.  0.3 us."""
-    return (torch.compiler.is_compiling() or _is_tracing() or _dispatch_modes() > 0
-            or _functorch_level() is not None)
-
-
+_is_compiling = torch.compiler.is_compiling
 _is_tracing = torch._C._is_tracing
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _functorch_level = torch._C._functorch.maybe_current_level
@@ -394,6 +389,7 @@ def wants_grad(*tensors) -> bool:
 # device-to-host copy when the caller asks -- so the ops never synchronise.
 STATUS_SLOTS = ("selective_scan", "state_update", "chunk_scan", "ss2d_scan", "causal_conv1d",
                 "causal_conv1d_update", "gated_rmsnorm", "selftest", "add_rmsnorm", "int8_linear", "gated_recurrence")
+_SLOT_BYTES = {op: 4 * i for i, op in enumerate(STATUS_SLOTS)}
 _status = {}
 
 
@@ -408,8 +404,7 @@ def _status_buffer(device: torch.device) -> torch.Tensor:
 
 def status_word(device: torch.device, op: str) -> int:
     """Device address of ``op``'s status word on ``device`` (for params.status)."""
-    buf = _status_buffer(device)
-    return buf.data_ptr() + 4 * STATUS_SLOTS.index(op)
+    return _status_buffer(device).data_ptr() + _SLOT_BYTES[op]
 
 
 def check_errors(device=None) -> None:
