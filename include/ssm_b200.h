@@ -587,7 +587,8 @@ int ssm_int8_linear_fwd(const ssm_int8_linear_params* p, void* stream);
  *   states : fp32, states_bytes of ssm_gated_recurrence_sizes, written by the
  *            forward (NULL: not saved) and read by the backward
  * z, dfinal, dinitial and dlower may be NULL.  The backward takes a workspace of
- * workspace_bytes.  A state that is not finite does not pass a reset.
+ * workspace_bytes.  Neither a state that is not finite nor a NaN gate passes a
+ * reset, forward or backward.
  * ------------------------------------------------------------------------- */
 typedef struct ssm_gated_recurrence_params {
     int64_t batch, length, dim;

@@ -8,17 +8,14 @@ pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
 
 
-@pytest.mark.parametrize("through_ops", [False, True])
 @pytest.mark.parametrize("stream", [None, BF16, F32])
-@pytest.mark.parametrize("shape", [(0, 64), (2, 0, 64), (0, 77)])
+@pytest.mark.parametrize("shape,through_ops", [((0, 64), False), ((2, 0, 64), False), ((0, 77), False), ((0, 64), True)])
 def test_norm(shape, stream, through_ops):
     from metal_kernelops_b200 import cv
     x = torch.empty(shape, device="cuda", dtype=BF16, requires_grad=True)
     res = None if stream is None else torch.empty(shape, device="cuda", dtype=stream, requires_grad=True)
     w = torch.ones(shape[-1], device="cuda", requires_grad=True)
     if through_ops:
-        if len(shape) > 2:
-            pytest.skip("the registered op takes rows")
         y, s, _ = torch.ops.b200ssm.add_rmsnorm_fwd(x, w, res, 1e-5, True)
     else:
         y, s = cv.add_rmsnorm(x, w, res)
